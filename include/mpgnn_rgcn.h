@@ -281,6 +281,68 @@ int32_t mpgnn_linear_logsoftmax_bwd(const float* grad_logp, const float* logp, c
 int32_t mpgnn_linear_dgrad_relu_in(const float* grad_out, int64_t N, int32_t O, const float* weight, int32_t F,
                                    const float* x, float* grad_x, void* stream);
 
+/* --- operators over fp32, bf16 and fp16 tensors ---------------------------------------
+ * Sums, statistics and matrix accumulators are fp32 or wider; a 16-bit result is rounded once. */
+enum mpgnn_dtype { MPGNN_F32 = 0, MPGNN_BF16 = 1, MPGNN_F16 = 2 };
+
+/* Layer norm over the last dimension (torch.nn.LayerNorm over node embeddings, as a model stacks
+ * it between the layers of model.py:144-146 / 211-215): y = (x - mean) * rstd * weight + bias with
+ * rstd = 1 / sqrt(mean((x - mean)^2) + eps). x: `rows` rows of `width` elements, x_pitch elements
+ * apart (a column slice needs no copy); y contiguous. weight / bias: [width] of the same type or
+ * fp32 (wdtype), or NULL (1 and 0). mean / rstd: [rows] fp32 for the backward, or both NULL. */
+int32_t mpgnn_layer_norm_fwd(const void* x, int64_t rows, int64_t width, int64_t x_pitch, int32_t dtype,
+                             const void* weight, const void* bias, int32_t wdtype, double eps, void* y, float* mean,
+                             float* rstd, void* stream);
+/* Its backward: dx (contiguous), dweight, dbias (wdtype; zeros for rows = 0), each or NULL. The
+ * parameters' gradients are fp32 partial rows per workgroup in `workspace` (needed if either is
+ * wanted), added in a fixed order: bitwise repeatable. */
+int32_t mpgnn_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t width, int64_t* bytes);
+int32_t mpgnn_layer_norm_bwd(const void* dy, int64_t dy_pitch, const void* x, int64_t x_pitch, int64_t rows,
+                             int64_t width, int32_t dtype, const void* weight, int32_t wdtype, const float* mean,
+                             const float* rstd, void* dx, void* dweight, void* dbias, void* workspace, void* stream);
+
+/* Matrix products grouped by type, relation or expert over groups of ragged sizes (the per-relation
+ * transform of mp_rgcn_layer.py:249-258 on its own, for any rows sorted by group): group g owns rows
+ * [group_ptr[g], group_ptr[g + 1]) of x and the matrix weight[g] of [groups, k, n].
+ *   fwd    out[i] = x[i] @ weight[g] + bias[g]   (bias [groups, n] or NULL)
+ *   dgrad  dx[i] = dy[i] @ weight[g]^T
+ *   wgrad  dweight[g] = x_g^T @ dy_g, dbias[g] = column sums of dy_g (dbias may be NULL)
+ * group_ptr: [groups + 1] int32 or int64 (ptr_bits) on the DEVICE, non-decreasing; its values are clamped
+ * to [0, rows], so that none leads outside the tensors, but a decreasing one makes groups overlap and
+ * their rows undefined. Rows in no group (before group_ptr[0], from group_ptr[groups] on) give zero
+ * rows of out and dx and take no part in the gradients; an empty group's dweight and dbias are zero.
+ * x / dy rows lie x_pitch / dy_pitch elements apart; all else is contiguous, aligned to its elements.
+ * fp32 operands run as exact three-way bf16 splits (six products, fp32 accumulation). */
+int32_t mpgnn_grouped_linear_fwd(const void* x, int64_t rows, int64_t x_pitch, int32_t dtype, const void* weight,
+                                 int64_t groups, int64_t k, int64_t n, const void* bias, const void* group_ptr,
+                                 int32_t ptr_bits, void* out, void* stream);
+int32_t mpgnn_grouped_linear_dgrad(const void* dy, int64_t rows, int64_t dy_pitch, int32_t dtype, const void* weight,
+                                   int64_t groups, int64_t k, int64_t n, const void* group_ptr, int32_t ptr_bits,
+                                   void* dx, void* stream);
+int32_t mpgnn_grouped_linear_wgrad_workspace_bytes(int64_t rows, int64_t groups, int64_t k, int64_t n, int64_t* bytes);
+int32_t mpgnn_grouped_linear_wgrad(const void* x, int64_t x_pitch, const void* dy, int64_t dy_pitch, int64_t rows,
+                                   int32_t dtype, int64_t groups, int64_t k, int64_t n, const void* group_ptr,
+                                   int32_t ptr_bits, void* dweight, void* dbias, void* workspace, void* stream);
+
+/* The global norm over a list of gradient tensors (the 2-norm of all their elements, or the largest
+ * |element|) -> *norm, and, if the tensors carry `out`, out = grad * min(1, max_norm / (norm + 1e-6))
+ * rounded once (out may be grad: in place; other overlaps are not allowed). What a loop runs
+ * between loss.backward() and optimizer.step() (main.py:1078-1079 has no clipping). Squares are
+ * summed in double in a fixed order: bitwise repeatable, no overflow. A NaN or infinite gradient
+ * gives the norm and the products that the formula gives. No host synchronisation; the tensor list
+ * is read before the call returns. */
+enum mpgnn_norm_kind { MPGNN_NORM_2 = 2, MPGNN_NORM_INF = 0 };
+typedef struct mpgnn_clip_tensor {
+    const void* grad; /* device, contiguous, aligned to its elements */
+    void* out;        /* NULL in every tensor: the norm alone */
+    int64_t numel;
+    int32_t dtype;
+    int32_t reserved;
+} mpgnn_clip_tensor;
+int32_t mpgnn_clip_workspace_bytes(int32_t n, int64_t* bytes);
+int32_t mpgnn_clip_by_global_norm(const mpgnn_clip_tensor* tensors, int32_t n, int32_t norm_kind, double max_norm,
+                                  float* norm, void* workspace, void* stream);
+
 /* The loops' optimizer step (Adam(lr=0.01, weight_decay=5e-4), main.py:1119 / main_rgcn.py:454)
  * over n <= 24 fp32 parameter tensors in ONE launch, replacing torch.optim.Adam(fused=True)'s
  * _foreach_add_(steps, 1) + _fused_adam_ pair: for each tensor, step += 1 (float, device

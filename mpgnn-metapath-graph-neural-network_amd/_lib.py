@@ -62,6 +62,12 @@ class AdamTensor(ctypes.Structure):
                 ("exp_avg_sq", ctypes.c_void_p), ("step", ctypes.c_void_p), ("numel", ctypes.c_int64)]
 
 
+class ClipTensor(ctypes.Structure):
+    """mpgnn_clip_tensor of include/mpgnn_rgcn.h."""
+    _fields_ = [("grad", ctypes.c_void_p), ("out", ctypes.c_void_p), ("numel", ctypes.c_int64),
+                ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
 # (name, restype, argtypes) — exactly the symbols of include/mpgnn_rgcn.h
 _P = ctypes.c_void_p
 _I32, _I64 = ctypes.c_int32, ctypes.c_int64
@@ -104,6 +110,15 @@ SIGNATURES = [
     ("mpgnn_linear_dgrad_relu_in", _I32, [_P, _I64, _I32, _P, _I32, _P, _P, _P]),
     ("mpgnn_linear_logsoftmax_bwd_workspace_bytes", _I32, [_I64, _I32, _I32, _PI64]),
     ("mpgnn_linear_logsoftmax_bwd", _I32, [_P, _P, _P, _I64, _I32, _I32, _P, _P, _P, _P, _P, _P, _P]),
+    ("mpgnn_layer_norm_fwd", _I32, [_P, _I64, _I64, _I64, _I32, _P, _P, _I32, ctypes.c_double, _P, _P, _P, _P]),
+    ("mpgnn_layer_norm_bwd_workspace_bytes", _I32, [_I64, _I64, _PI64]),
+    ("mpgnn_layer_norm_bwd", _I32, [_P, _I64, _P, _I64, _I64, _I64, _I32, _P, _I32, _P, _P, _P, _P, _P, _P, _P]),
+    ("mpgnn_grouped_linear_fwd", _I32, [_P, _I64, _I64, _I32, _P, _I64, _I64, _I64, _P, _P, _I32, _P, _P]),
+    ("mpgnn_grouped_linear_dgrad", _I32, [_P, _I64, _I64, _I32, _P, _I64, _I64, _I64, _P, _I32, _P, _P]),
+    ("mpgnn_grouped_linear_wgrad_workspace_bytes", _I32, [_I64, _I64, _I64, _I64, _PI64]),
+    ("mpgnn_grouped_linear_wgrad", _I32, [_P, _I64, _P, _I64, _I64, _I32, _I64, _I64, _I64, _P, _I32, _P, _P, _P, _P]),
+    ("mpgnn_clip_workspace_bytes", _I32, [_I32, _PI64]),
+    ("mpgnn_clip_by_global_norm", _I32, [_P, _I32, _I32, ctypes.c_double, _P, _P, _P]),
     ("mpgnn_adam_step", _I32, [ctypes.POINTER(AdamTensor), _I32, ctypes.c_double, ctypes.c_double, ctypes.c_double,
                                 ctypes.c_double, ctypes.c_double, _P, _P]),
     ("mpgnn_score_argmax", _I32, [_P, _I64, _P, _P, _P, _I64, _P, _P, _P, _P]),
@@ -138,6 +153,8 @@ KERNEL_KINDS = {"seg_fwd": 0, "row_fwd": 1, "seg_dgrad": 2, "row_dx": 3, "outer"
                 "piece": 7, "final": 8}
 OPT_EXACT_ORDER = 0
 OPT_ADAM_CONTRACT = 40
+F32, BF16, F16 = 0, 1, 2  # mpgnn_dtype
+NORM_2, NORM_INF = 2, 0  # mpgnn_norm_kind
 ACT_NONE, ACT_RELU, ACT_LOG_SOFTMAX = 0, 1, 2
 
 

@@ -1,0 +1,642 @@
+// Matrix products grouped by type, relation or expert, over groups of ragged sizes:
+//   forward          y[i]  = x[i] @ W[g] + b[g]          for the rows i of group g
+//   input gradient   dx[i] = dy[i] @ W[g]^T
+//   weight gradient  dW[g] = x_g^T @ dy_g,  db[g] = the column sums of dy_g
+// with x [M, K] sorted by group, group g owning rows [ptr[g], ptr[g + 1]), W [G, K, N], and ptr on
+// the device: no size is known to the host, so each launch has a workgroup for every tile that
+// there could be (rows / tile + groups), and a workgroup finds its tile by a scan over ptr.
+//
+// One kernel computes D[r][n] = sum_c R(r, c) * B(n, c) in tiles on the matrix cores
+// (v_mfma_f32_16x16x32, fp32 accumulators) with either operand stored along c or across it:
+//   forward          R = x (along c = k)       B = W  (across: n runs fastest)
+//   input gradient   R = dy (along c = n)      B = W  (along: c = n runs fastest)
+//   weight gradient  R = x (across: c = rows)  B = dy (across)
+// An operand stored along c goes to LDS as [index][c] and its fragments are 16-byte reads; one
+// stored across goes as [c][index] and its fragments are transposed reads (ds_read_b64_tr_b16: a
+// 16-lane group reads 4 c x 16 indices, lane i receives index i). Both layouts place 16-byte
+// (32-byte) pieces by an exclusive-or with the row, which keeps each read's lanes on distinct banks.
+// B is the first matrix operand, so that a lane ends up with four neighbouring columns of a row.
+//
+// fp32 operands run on the bf16 matrix cores: an exact split of each value in three bf16 pieces
+// and the six products of at least 2^-16 of the full one, which leaves an error of fp32's own
+// size at 16/6 of the fp32 matrix rate. An element whose pieces overflow or are not finite gives a
+// result that is not finite; such results are computed again from the operands in fp32, so that
+// infinities and NaN come out as a sum of products has them.
+#include <algorithm>
+
+#include "num_types.h"
+
+namespace mpgnn {
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kGlThreads = 256;
+
+enum Layout { ALONG, ACROSS };  // c fastest, or the index fastest
+
+struct GroupedArgs {
+    const void* r;      // rows operand
+    const void* b;      // columns operand
+    void* out;
+    const void* bias;   // forward: [G][cols] or null
+    const void* ptr;    // [G + 1] int32 or int64
+    float* slabs;       // weight gradient: [items][K * N (+ N)] partials of groups cut in chunks
+    void* dbias;        // weight gradient: [G][cols] or null
+    int64_t rows;       // M
+    int64_t r_pitch, b_pitch;
+    int64_t b_group;    // elements from one group's B to the next (0: B has no groups)
+    int32_t groups;
+    int32_t ptr64;
+    int32_t cc;         // forward, input gradient: length of c
+    int32_t out_rows;   // weight gradient: K
+    int32_t cols;       // columns of the output
+    int32_t col_tiles, row_tiles;
+    int32_t chunk;      // weight gradient: rows of a chunk
+    int64_t items;      // weight gradient: slabs there are room for
+};
+
+// 8 values of c of one index from a tile stored across: two transposed reads of 4 c x 16 indices
+template <typename V8, typename T>
+__device__ __forceinline__ V8 read_across(const T* lo, const T* hi) {
+    typedef __attribute__((address_space(3))) i16x4 lds4;
+    const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)lo);
+    const i16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)hi);
+    return __builtin_bit_cast(V8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+template <typename T>
+struct Frag;
+template <>
+struct Frag<__bf16> {
+    typedef bf16x8 type;
+    static __device__ __forceinline__ f32x4 mfma(type a, type b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+};
+template <>
+struct Frag<_Float16> {
+    typedef f16x8 type;
+    static __device__ __forceinline__ f32x4 mfma(type a, type b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    }
+};
+
+// How an element type is staged: 16-bit as itself, fp32 as three bf16 planes.
+template <typename T>
+struct Stage {
+    typedef T elem;
+    static constexpr int planes = 1, bk = 64;
+};
+template <>
+struct Stage<float> {
+    typedef __bf16 elem;
+    static constexpr int planes = 3, bk = 32;
+};
+
+// ---------------------------------------------------------------------------------------
+// groups and tiles
+// ---------------------------------------------------------------------------------------
+__device__ __forceinline__ int64_t ptr_at(const GroupedArgs& a, int g) {
+    const int64_t v = a.ptr64 ? ((const int64_t*)a.ptr)[g] : (int64_t)((const int32_t*)a.ptr)[g];
+    return v < 0 ? 0 : v > a.rows ? a.rows : v;  // no ptr, however wrong, leads outside the tensors
+}
+
+struct Item {
+    int group;    // -1: none; groups: rows that belong to no group
+    int part;     // which tile (chunk) of the group
+    int parts;    // of how many
+    int64_t lo, hi;
+};
+
+// Item `id` of the list of all groups' parts: each group has ceil(rows / size) of them, at least
+// `least`. With `rest`, the rows before ptr[0] and from ptr[G] on follow as two more groups.
+__device__ __forceinline__ Item find_item(const GroupedArgs& a, int64_t id, int size, int least, bool rest) {
+    __shared__ int64_t s_wave[kGlThreads / 64];
+    __shared__ Item s_item;
+    const int n = a.groups + (rest ? 2 : 0);
+    if (threadIdx.x == 0) s_item.group = -1;
+    int64_t base = 0;
+    for (int g0 = 0; g0 < n; g0 += kGlThreads) {
+        const int g = g0 + threadIdx.x;
+        int64_t lo = 0, hi = 0, parts = 0;
+        if (g < a.groups) {
+            lo = ptr_at(a, g);
+            hi = ptr_at(a, g + 1);
+            hi = hi < lo ? lo : hi;
+        } else if (g == a.groups) {
+            lo = ptr_at(a, a.groups);
+            hi = a.rows;
+        } else {
+            hi = ptr_at(a, 0);
+        }
+        if (g < n) {
+            parts = (hi - lo + size - 1) / size;
+            if (g < a.groups && parts < least) parts = least;
+        }
+        int64_t sum = parts;  // inclusive scan over the wave
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int64_t v = __shfl_up(sum, d, 64);
+            if ((int)(threadIdx.x % 64) >= d) sum += v;
+        }
+        if (threadIdx.x % 64 == 63) s_wave[threadIdx.x / 64] = sum;
+        __syncthreads();
+        int64_t before = base;
+        for (int w = 0; w < kGlThreads / 64; ++w) {
+            if (w < (int)(threadIdx.x / 64)) before += s_wave[w];
+            base += s_wave[w];
+        }
+        const int64_t first = before + sum - parts;
+        if (id >= first && id < first + parts)
+            s_item = Item{g < a.groups ? g : a.groups, (int)(id - first), (int)parts, lo, hi};
+        __syncthreads();
+        if (base > id) break;
+    }
+    __syncthreads();
+    return s_item;
+}
+
+// ---------------------------------------------------------------------------------------
+// staging: 8 elements of an operand, in memory (raw) and in LDS (planes)
+// ---------------------------------------------------------------------------------------
+template <typename T>
+struct Raw {
+    u32x4 v[sizeof(T) / 2];
+};
+
+// `valid` of 8 elements at p (any alignment of an element: the hardware's loads need no more)
+template <typename T>
+__device__ __forceinline__ Raw<T> load8(const T* p, int valid) {
+    Raw<T> r;
+    if (valid >= 8) {
+        __builtin_memcpy(&r, p, sizeof(r));
+    } else {
+        T e[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = i < valid ? p[i] : (T)0.0f;
+        __builtin_memcpy(&r, e, sizeof(r));
+    }
+    return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(typename Stage<T>::elem* dst, int plane_size, const Raw<T>& r) {
+    if constexpr (sizeof(T) == 2) {
+        *reinterpret_cast<u32x4*>(dst) = r.v[0];
+    } else {
+        float f[8];
+        __builtin_memcpy(f, &r, sizeof(f));
+        bf16x8 p0, p1, p2;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            p0[i] = (__bf16)f[i];
+            const float d = f[i] - (float)p0[i];
+            p1[i] = (__bf16)d;
+            p2[i] = (__bf16)(d - (float)p1[i]);
+        }
+        *reinterpret_cast<bf16x8*>(dst) = p0;
+        *reinterpret_cast<bf16x8*>(dst + plane_size) = p1;
+        *reinterpret_cast<bf16x8*>(dst + 2 * plane_size) = p2;
+    }
+}
+
+// A tile of IDX indices x BK of c.
+template <typename T, Layout L, int IDX>
+struct Tile {
+    typedef typename Stage<T>::elem E;
+    static constexpr int BK = Stage<T>::bk;
+    static constexpr int plane = IDX * BK;                         // elements
+    static constexpr int chunks = IDX * BK / 8 / kGlThreads;       // 8-element pieces per thread
+    static_assert(chunks >= 1, "every thread stages a piece");
+
+    // piece n of a thread: (index, c) of its first element
+    static __device__ __forceinline__ void place(int n, int& idx, int& c) {
+        const int id = threadIdx.x + n * kGlThreads;
+        if constexpr (L == ALONG) {
+            idx = id / (BK / 8);
+            c = id % (BK / 8) * 8;
+        } else {
+            c = id / (IDX / 8);
+            idx = id % (IDX / 8) * 8;
+        }
+    }
+    static __device__ __forceinline__ int offset(int idx, int c) {
+        if constexpr (L == ALONG) {
+            const int q = BK == 64 ? (c / 8) ^ (idx & 7) : (c / 8) ^ ((idx >> 1) & 3);
+            return idx * BK + q * 8 + c % 8;
+        } else {
+            constexpr int m = IDX / 16 < 8 ? IDX / 16 - 1 : 7;
+            return c * IDX + ((idx / 16) ^ (c & m)) * 16 + idx % 16;
+        }
+    }
+    // 8 values of c from c0 + 8 * (lane / 16) on, of index i0 + lane % 16
+    static __device__ __forceinline__ typename Frag<E>::type frag(const E* lds, int i0, int c0) {
+        const int lane = threadIdx.x % 64;
+        if constexpr (L == ALONG) {
+            return *reinterpret_cast<const typename Frag<E>::type*>(lds + offset(i0 + lane % 16, c0 + lane / 16 * 8));
+        } else {
+            constexpr int m = IDX / 16 < 8 ? IDX / 16 - 1 : 7;
+            const int c = c0 + lane / 16 * 8 + (lane % 16) / 4;
+            // rows c and c + 4 differ in the exclusive-or: two addresses
+            const E* lo = lds + c * IDX + ((i0 / 16) ^ (c & m)) * 16 + lane % 4 * 4;
+            const E* hi = lds + (c + 4) * IDX + ((i0 / 16) ^ ((c + 4) & m)) * 16 + lane % 4 * 4;
+            return read_across<typename Frag<E>::type>(lo, hi);
+        }
+    }
+    // the tile of `p` whose indices start at i0 (of i_n) and whose c at c0 (of c_n); outside: zero
+    static __device__ __forceinline__ void load(Raw<T> (&raw)[chunks], const T* p, int64_t pitch, int64_t i0,
+                                                int64_t i_n, int64_t c0, int64_t c_n) {
+#pragma unroll
+        for (int n = 0; n < chunks; ++n) {
+            int idx, c;
+            place(n, idx, c);
+            const int64_t i = i0 + idx, k = c0 + c;
+            const int64_t left = L == ALONG ? (i < i_n ? c_n - k : 0) : (k < c_n ? i_n - i : 0);
+            const int valid = left >= 8 ? 8 : left > 0 ? (int)left : 0;
+            raw[n] = load8<T>(valid ? p + (L == ALONG ? i * pitch + k : k * pitch + i) : p, valid);
+        }
+    }
+    static __device__ __forceinline__ void store(E* lds, const Raw<T> (&raw)[chunks]) {
+#pragma unroll
+        for (int n = 0; n < chunks; ++n) {
+            int idx, c;
+            place(n, idx, c);
+            store8<T>(lds + offset(idx, c), plane, raw[n]);
+        }
+    }
+};
+
+// ---------------------------------------------------------------------------------------
+// the tile product
+// ---------------------------------------------------------------------------------------
+template <typename T, Layout LR, Layout LB, int BR, int BN>
+struct Product {
+    typedef typename Stage<T>::elem E;
+    typedef Tile<T, LR, BR> TR;
+    typedef Tile<T, LB, BN> TB;
+    static constexpr int BK = Stage<T>::bk, P = Stage<T>::planes;
+    static constexpr int waves_r = BR >= 128 ? 2 : 1, waves_n = 4 / waves_r;
+    static constexpr int WR = BR / waves_r, WN = BN / waves_n;
+    static constexpr int NR = WR / 16, NN = WN / 16;
+    static constexpr int lds_elems = P * (TR::plane + TB::plane);
+
+    static __device__ __forceinline__ void step(const E* lr, const E* lb, f32x4 (&acc)[NR][NN]) {
+        const int wave = threadIdx.x / 64;
+        const int r0 = wave / waves_n * WR, n0 = wave % waves_n * WN;
+#pragma unroll
+        for (int c = 0; c < BK; c += 32) {
+            typename Frag<E>::type fb[P][NN];
+#pragma unroll
+            for (int p = 0; p < P; ++p)
+#pragma unroll
+                for (int j = 0; j < NN; ++j) fb[p][j] = TB::frag(lb + p * TB::plane, n0 + j * 16, c);
+#pragma unroll
+            for (int i = 0; i < NR; ++i) {
+                typename Frag<E>::type fr[P];
+#pragma unroll
+                for (int p = 0; p < P; ++p) fr[p] = TR::frag(lr + p * TR::plane, r0 + i * 16, c);
+#pragma unroll
+                for (int j = 0; j < NN; ++j) {
+                    if constexpr (P == 1) {
+                        acc[i][j] = Frag<E>::mfma(fb[0][j], fr[0], acc[i][j]);
+                    } else {  // smallest products first
+                        acc[i][j] = Frag<E>::mfma(fb[2][j], fr[0], acc[i][j]);
+                        acc[i][j] = Frag<E>::mfma(fb[1][j], fr[1], acc[i][j]);
+                        acc[i][j] = Frag<E>::mfma(fb[0][j], fr[2], acc[i][j]);
+                        acc[i][j] = Frag<E>::mfma(fb[1][j], fr[0], acc[i][j]);
+                        acc[i][j] = Frag<E>::mfma(fb[0][j], fr[1], acc[i][j]);
+                        acc[i][j] = Frag<E>::mfma(fb[0][j], fr[0], acc[i][j]);
+                    }
+                }
+            }
+        }
+    }
+
+    // acc += R[r0.., c] * B[n0.., c] over c in [c_lo, c_hi). `seen(raw of B's tile)` sees each of them.
+    template <typename F>
+    static __device__ __forceinline__ void run(E* lds, f32x4 (&acc)[NR][NN], const T* r, int64_t r_pitch, int64_t r0,
+                                               int64_t r_n, const T* b, int64_t b_pitch, int64_t n0, int64_t b_n,
+                                               int64_t c_lo, int64_t c_hi, F&& seen) {
+        E* lr = lds;
+        E* lb = lds + P * TR::plane;
+        Raw<T> rr[TR::chunks], rb[TB::chunks];
+        if (c_lo >= c_hi) return;
+        TR::load(rr, r, r_pitch, r0, r_n, c_lo, c_hi);
+        TB::load(rb, b, b_pitch, n0, b_n, c_lo, c_hi);
+        for (int64_t c = c_lo; c < c_hi; c += BK) {
+            __syncthreads();  // the last step's reads are done
+            TR::store(lr, rr);
+            TB::store(lb, rb);
+            seen(rb);
+            __syncthreads();
+            if (c + BK < c_hi) {
+                TR::load(rr, r, r_pitch, r0, r_n, c + BK, c_hi);
+                TB::load(rb, b, b_pitch, n0, b_n, c + BK, c_hi);
+            }
+            step(lr, lb, acc);
+        }
+    }
+
+    // f(row, column, its four results) for each quadruple that this lane holds
+    template <typename F>
+    static __device__ __forceinline__ void each(f32x4 (&acc)[NR][NN], F&& f) {
+        const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+        const int r0 = wave / waves_n * WR, n0 = wave % waves_n * WN;
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+#pragma unroll
+            for (int j = 0; j < NN; ++j) f(r0 + i * 16 + lane % 16, n0 + j * 16 + lane / 16 * 4, acc[i][j]);
+    }
+};
+
+__device__ __forceinline__ bool finite(float v) { return __builtin_fabsf(v) <= 3.402823466e38f; }
+
+template <typename T>
+__device__ __forceinline__ void store4(T* p, const f32x4& v, int valid) {
+    if (valid >= 4) {
+        T e[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) e[k] = (T)v[k];
+        __builtin_memcpy(p, e, sizeof(e));
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (k < valid) p[k] = (T)v[k];
+    }
+}
+
+// forward (LB = ACROSS) and input gradient (LB = ALONG): a workgroup per row tile and column tile
+template <typename T, Layout LB, int BR, int BN>
+__global__ __launch_bounds__(kGlThreads) void grouped_rows_kernel(GroupedArgs a) {
+    typedef Product<T, ALONG, LB, BR, BN> X;
+    __shared__ __attribute__((aligned(16))) typename X::E lds[X::lds_elems];
+    const Item it = find_item(a, blockIdx.x / a.col_tiles, BR, 0, true);
+    if (it.group < 0) return;
+    const int64_t n0 = (int64_t)(blockIdx.x % a.col_tiles) * BN;
+    const int64_t r0 = it.lo + (int64_t)it.part * BR;
+    f32x4 acc[X::NR][X::NN] = {};
+    const bool owned = it.group < a.groups;
+    const T* r = (const T*)a.r;
+    const T* b = (const T*)a.b + (owned ? (int64_t)it.group * a.b_group : 0);
+    if (owned)
+        X::run(lds, acc, r, a.r_pitch, r0, it.hi, b, a.b_pitch, n0, a.cols, 0, a.cc, [](auto&) {});
+    const T* bias = owned && a.bias ? (const T*)a.bias + (int64_t)it.group * a.cols : nullptr;
+    X::each(acc, [&](int ir, int in, f32x4& v) {
+        const int64_t row = r0 + ir, col = n0 + in;
+        if (row >= it.hi || col >= a.cols) return;
+        const int valid = a.cols - col < 4 ? (int)(a.cols - col) : 4;
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (finite(v[k]) || k >= valid || !owned) continue;
+                float s = 0.0f;
+                for (int c = 0; c < a.cc; ++c)
+                    s = __builtin_fmaf(r[row * a.r_pitch + c],
+                                       LB == ALONG ? b[(col + k) * a.b_pitch + c] : b[c * a.b_pitch + col + k], s);
+                v[k] = s;
+            }
+        }
+        if (bias) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (k < valid) v[k] += (float)bias[col + k];
+        }
+        store4<T>((T*)a.out + row * a.cols + col, v, valid);
+    });
+}
+
+// weight gradient: a workgroup per chunk of a group's rows and tile of the weight. A group of one
+// chunk is written as it is; the chunks of a longer one leave fp32 slabs for the kernel below.
+template <typename T, int BR, int BN>
+__global__ __launch_bounds__(kGlThreads) void grouped_wgrad_kernel(GroupedArgs a) {
+    typedef Product<T, ACROSS, ACROSS, BR, BN> X;
+    __shared__ __attribute__((aligned(16))) typename X::E lds[X::lds_elems];
+    const int tiles = a.row_tiles * a.col_tiles;
+    const int64_t id = blockIdx.x / tiles;
+    const int tile = blockIdx.x % tiles;
+    const Item it = find_item(a, id, a.chunk, 1, false);
+    if (it.group < 0) return;
+    const int64_t r0 = (int64_t)(tile / a.col_tiles) * BR, n0 = (int64_t)(tile % a.col_tiles) * BN;
+    const int64_t c_lo = it.lo + (int64_t)it.part * a.chunk;
+    const int64_t c_hi = c_lo + a.chunk < it.hi ? c_lo + a.chunk : it.hi;
+    f32x4 acc[X::NR][X::NN] = {};
+    float col_sum[8] = {};  // of the columns that this thread stages: the same in every piece
+    const bool want_b = a.dbias && r0 == 0;
+    const T* r = (const T*)a.r;
+    const T* b = (const T*)a.b;
+    X::run(lds, acc, r, a.r_pitch, r0, a.out_rows, b, a.b_pitch, n0, a.cols, c_lo, c_hi, [&](auto& raw) {
+        if (!want_b) return;
+#pragma unroll
+        for (int n = 0; n < X::TB::chunks; ++n) {
+            T e[8];
+            __builtin_memcpy(e, &raw[n], sizeof(e));
+#pragma unroll
+            for (int k = 0; k < 8; ++k) col_sum[k] += (float)e[k];
+        }
+    });
+    const int64_t size = (int64_t)a.out_rows * a.cols;
+    const int64_t slab = size + (a.dbias ? a.cols : 0);
+    float* part = it.parts > 1 ? a.slabs + id * slab : nullptr;
+    X::each(acc, [&](int ir, int in, f32x4& v) {
+        const int64_t row = r0 + ir, col = n0 + in;
+        if (row >= a.out_rows || col >= a.cols) return;
+        const int valid = a.cols - col < 4 ? (int)(a.cols - col) : 4;
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (finite(v[k]) || k >= valid) continue;
+                float s = 0.0f;
+                for (int64_t c = c_lo; c < c_hi; ++c)
+                    s = __builtin_fmaf(r[c * a.r_pitch + row], b[c * a.b_pitch + col + k], s);
+                v[k] = s;
+            }
+        }
+        if (part) store4<float>(part + row * a.cols + col, v, valid);
+        else store4<T>((T*)a.out + (int64_t)it.group * size + row * a.cols + col, v, valid);
+    });
+    if (!want_b) return;
+    // the threads that staged the same columns, in order
+    constexpr int teams = kGlThreads / (BN / 8);
+    static_assert(X::TB::chunks * kGlThreads * 8 == BN * X::BK, "a thread's pieces share their columns");
+    float* sums = reinterpret_cast<float*>(lds);
+    static_assert(sizeof(lds) >= teams * BN * sizeof(float), "the column sums fit the stage");
+    __syncthreads();
+    const int team = threadIdx.x / (BN / 8), c8 = threadIdx.x % (BN / 8) * 8;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sums[team * BN + c8 + k] = col_sum[k];
+    __syncthreads();
+    for (int c = threadIdx.x; c < BN && n0 + c < a.cols; c += kGlThreads) {
+        float s = sums[c];
+        for (int q = 1; q < teams; ++q) s += sums[q * BN + c];
+        if (part) part[size + n0 + c] = s;
+        else ((T*)a.dbias)[(int64_t)it.group * a.cols + n0 + c] = (T)s;
+    }
+}
+
+// dW[g] (and db[g]) of the groups cut in chunks: their slabs added in order
+template <typename T>
+__global__ __launch_bounds__(kGlThreads) void grouped_slabs_kernel(GroupedArgs a, int pieces) {
+    __shared__ int64_t s_first;
+    const int g = blockIdx.x / pieces;
+    const int64_t lo = ptr_at(a, g), hi = ptr_at(a, g + 1);
+    if (hi - lo <= a.chunk) return;
+    int64_t parts = (hi - lo + a.chunk - 1) / a.chunk;
+    // items before this group
+    if (threadIdx.x == 0) s_first = 0;
+    __syncthreads();
+    int64_t before = 0;
+    for (int q = threadIdx.x; q < g; q += kGlThreads) {
+        const int64_t l = ptr_at(a, q), h = ptr_at(a, q + 1);
+        const int64_t n = (h - l + a.chunk - 1) / a.chunk;
+        before += n < 1 ? 1 : n;
+    }
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) before += __shfl_xor(before, d, 64);
+    if (threadIdx.x % 64 == 0) atomicAdd((unsigned long long*)&s_first, (unsigned long long)before);  // whole numbers
+    __syncthreads();
+    const int64_t size = (int64_t)a.out_rows * a.cols, slab = size + (a.dbias ? a.cols : 0);
+    const float* p = a.slabs + s_first * slab;
+    parts = min(parts, a.items - s_first);  // short only where ptr decreases and groups overlap
+    if (parts < 1) return;
+    for (int64_t e = (int64_t)(blockIdx.x % pieces) * kGlThreads + threadIdx.x; e < slab;
+         e += (int64_t)pieces * kGlThreads) {
+        float s = p[e];
+        for (int k = 1; k < parts; ++k) s += p[k * slab + e];
+        if (e < size) ((T*)a.out)[(int64_t)g * size + e] = (T)s;
+        else ((T*)a.dbias)[(int64_t)g * a.cols + e - size] = (T)s;
+    }
+}
+
+// ---------------------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------------------
+constexpr int kTile = 128;
+
+// Rows of a chunk of the weight gradient: whole groups where the weight alone has tiles enough to
+// fill the chip, else as many rows as leave about four workgroups per CU.
+int64_t wgrad_chunk(int64_t rows, int64_t groups, int64_t k, int64_t n) {
+    const int64_t tiles = ((k + kTile - 1) / kTile) * ((n + kTile - 1) / kTile);
+    const int64_t want = 1024 / tiles;  // chunks over all groups
+    if (want <= groups || rows == 0) return std::max<int64_t>(rows, 1);
+    const int64_t c = (rows + want - 1) / want;
+    return std::max<int64_t>(256, (c + 63) / 64 * 64);
+}
+
+int64_t wgrad_items(int64_t rows, int64_t groups, int64_t chunk) { return rows / chunk + groups; }
+
+int32_t check_grouped(int64_t rows, int64_t groups, int64_t k, int64_t n, int32_t dtype, int32_t ptr_bits) {
+    if (rows < 0 || groups < 1 || k < 1 || n < 1)
+        return arg_error("grouped linear: rows < 0, or fewer than one group, input or output column");
+    if (!dtype_bytes(dtype)) return arg_error("grouped linear: unknown dtype");
+    if (ptr_bits != 32 && ptr_bits != 64) return arg_error("grouped linear: group_ptr is int32 or int64");
+    if (k > (1 << 24) || n > (1 << 24) || groups > (1 << 24) || rows > (int64_t{1} << 40))
+        return unsupported("grouped linear: more than 2^24 columns or groups, or 2^40 rows");
+    return MPGNN_OK;
+}
+
+template <typename T>
+int32_t rows_product(GroupedArgs a, bool dgrad, hipStream_t strm) {
+    a.col_tiles = (a.cols + kTile - 1) / kTile;
+    const int64_t blocks = (a.rows / kTile + a.groups + 2) * a.col_tiles;
+    if (blocks > INT32_MAX) return unsupported("grouped linear: more than 2^31 tiles");
+    if (dgrad)
+        hipLaunchKernelGGL((grouped_rows_kernel<T, ALONG, kTile, kTile>), dim3((unsigned)blocks), dim3(kGlThreads), 0,
+                           strm, a);
+    else
+        hipLaunchKernelGGL((grouped_rows_kernel<T, ACROSS, kTile, kTile>), dim3((unsigned)blocks), dim3(kGlThreads), 0,
+                           strm, a);
+    return launch_status("grouped linear: the launch failed");
+}
+
+int32_t rows_by_type(const GroupedArgs& a, int32_t dtype, bool dgrad, hipStream_t strm) {
+    if (a.rows == 0) return MPGNN_OK;
+    if (dtype == MPGNN_F32) return rows_product<float>(a, dgrad, strm);
+    return dtype == MPGNN_BF16 ? rows_product<__bf16>(a, dgrad, strm) : rows_product<_Float16>(a, dgrad, strm);
+}
+
+template <typename T>
+int32_t wgrad_product(GroupedArgs a, hipStream_t strm) {
+    a.row_tiles = (a.out_rows + kTile - 1) / kTile;
+    a.col_tiles = (a.cols + kTile - 1) / kTile;
+    a.items = wgrad_items(a.rows, a.groups, a.chunk);
+    const int64_t blocks = a.items * a.row_tiles * a.col_tiles;
+    if (blocks > INT32_MAX) return unsupported("grouped linear: more than 2^31 tiles");
+    hipLaunchKernelGGL((grouped_wgrad_kernel<T, kTile, kTile>), dim3((unsigned)blocks), dim3(kGlThreads), 0, strm, a);
+    if (a.rows > a.chunk) {
+        const int64_t slab = (int64_t)a.out_rows * a.cols + a.cols;
+        const int pieces = (int)std::min<int64_t>(64, (slab + kGlThreads * 4 - 1) / (kGlThreads * 4));
+        hipLaunchKernelGGL(grouped_slabs_kernel<T>, dim3((unsigned)a.groups * pieces), dim3(kGlThreads), 0, strm, a,
+                           pieces);
+    }
+    return launch_status("grouped linear: a launch failed");
+}
+
+}  // namespace
+}  // namespace mpgnn
+
+extern "C" int32_t mpgnn_grouped_linear_fwd(const void* x, int64_t rows, int64_t x_pitch, int32_t dtype,
+                                            const void* weight, int64_t groups, int64_t k, int64_t n, const void* bias,
+                                            const void* group_ptr, int32_t ptr_bits, void* out, void* stream) {
+    using namespace mpgnn;
+    int32_t st = check_grouped(rows, groups, k, n, dtype, ptr_bits);
+    if (st != MPGNN_OK) return st;
+    if (!weight || !group_ptr || (rows > 0 && (!x || !out)) || (rows > 1 && x_pitch < k))
+        return arg_error("mpgnn_grouped_linear_fwd: a null pointer, or x's row pitch is below its width");
+    GroupedArgs a{};
+    a.r = x; a.r_pitch = x_pitch; a.b = weight; a.b_pitch = n; a.b_group = k * n; a.out = out; a.bias = bias;
+    a.ptr = group_ptr; a.ptr64 = ptr_bits == 64; a.rows = rows; a.groups = (int32_t)groups; a.cc = (int32_t)k;
+    a.cols = (int32_t)n;
+    return rows_by_type(a, dtype, false, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int32_t mpgnn_grouped_linear_dgrad(const void* dy, int64_t rows, int64_t dy_pitch, int32_t dtype,
+                                              const void* weight, int64_t groups, int64_t k, int64_t n,
+                                              const void* group_ptr, int32_t ptr_bits, void* dx, void* stream) {
+    using namespace mpgnn;
+    int32_t st = check_grouped(rows, groups, k, n, dtype, ptr_bits);
+    if (st != MPGNN_OK) return st;
+    if (!weight || !group_ptr || (rows > 0 && (!dy || !dx)) || (rows > 1 && dy_pitch < n))
+        return arg_error("mpgnn_grouped_linear_dgrad: a null pointer, or dy's row pitch is below its width");
+    GroupedArgs a{};
+    a.r = dy; a.r_pitch = dy_pitch; a.b = weight; a.b_pitch = n; a.b_group = k * n; a.out = dx;
+    a.ptr = group_ptr; a.ptr64 = ptr_bits == 64; a.rows = rows; a.groups = (int32_t)groups; a.cc = (int32_t)n;
+    a.cols = (int32_t)k;
+    return rows_by_type(a, dtype, true, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int32_t mpgnn_grouped_linear_wgrad_workspace_bytes(int64_t rows, int64_t groups, int64_t k, int64_t n,
+                                                              int64_t* bytes) {
+    using namespace mpgnn;
+    int32_t st = check_grouped(rows, groups, k, n, MPGNN_F32, 64);
+    if (st != MPGNN_OK) return st;
+    if (!bytes) return arg_error("mpgnn_grouped_linear_wgrad_workspace_bytes: bytes is null");
+    const int64_t chunk = wgrad_chunk(rows, groups, k, n);
+    *bytes = rows > chunk ? wgrad_items(rows, groups, chunk) * (k * n + n) * (int64_t)sizeof(float) : 0;
+    return MPGNN_OK;
+}
+
+extern "C" int32_t mpgnn_grouped_linear_wgrad(const void* x, int64_t x_pitch, const void* dy, int64_t dy_pitch,
+                                              int64_t rows, int32_t dtype, int64_t groups, int64_t k, int64_t n,
+                                              const void* group_ptr, int32_t ptr_bits, void* dweight, void* dbias,
+                                              void* workspace, void* stream) {
+    using namespace mpgnn;
+    int32_t st = check_grouped(rows, groups, k, n, dtype, ptr_bits);
+    if (st != MPGNN_OK) return st;
+    if (!dweight || !group_ptr || (rows > 0 && (!x || !dy)) || (rows > 1 && (x_pitch < k || dy_pitch < n)))
+        return arg_error("mpgnn_grouped_linear_wgrad: a null pointer, or a row pitch below the width");
+    const int64_t chunk = wgrad_chunk(rows, groups, k, n);
+    if (rows > chunk && !workspace) return arg_error("mpgnn_grouped_linear_wgrad: no workspace");
+    if (chunk > INT32_MAX) return unsupported("mpgnn_grouped_linear_wgrad: over 2^31 rows");
+    GroupedArgs a{};
+    a.r = x; a.r_pitch = x_pitch; a.b = dy; a.b_pitch = dy_pitch; a.out = dweight; a.dbias = dbias;
+    a.slabs = static_cast<float*>(workspace); a.ptr = group_ptr; a.ptr64 = ptr_bits == 64; a.rows = rows;
+    a.groups = (int32_t)groups; a.out_rows = (int32_t)k; a.cols = (int32_t)n; a.chunk = (int32_t)chunk;
+    hipStream_t strm = static_cast<hipStream_t>(stream);
+    if (dtype == MPGNN_F32) return wgrad_product<float>(a, strm);
+    return dtype == MPGNN_BF16 ? wgrad_product<__bf16>(a, strm) : wgrad_product<_Float16>(a, strm);
+}

@@ -1,0 +1,494 @@
+// Layer norm over the last dimension, forward and backward:
+//   y  = xhat * w + b,   xhat = (x - mean) * rstd,   rstd = 1 / sqrt(mean((x - mean)^2) + eps)
+//   dx = rstd * (h - mean(h) - xhat * mean(h * xhat)),   h = dy * w
+//   dw = sum over rows of dy * xhat,   db = sum over rows of dy
+// Bound by memory: the forward reads x and writes y, the backward reads x and dy and writes dx.
+//
+// A row lies in the registers of TPR threads (16 to 64 lanes of a wave, or a whole workgroup), so
+// that it is read once: the mean first, then the squared differences from it (a sum of squares
+// minus a squared mean would lose the variance of rows far from zero). All sums are fp32 or wider.
+// The backward's threads keep their columns' dw and db over all rows that their workgroup takes
+// and write one fp32 partial row per workgroup; a second kernel adds the partial rows in order
+// (in double), so gradients do not change from run to run. fp32 inputs keep a compensation term
+// beside each of these sums, since one thread adds hundreds of rows.
+#include <algorithm>
+
+#include "num_types.h"
+
+namespace mpgnn {
+namespace {
+
+struct NormArgs {
+    const void* x;
+    const void* dy;
+    void* out;         // y, or dx
+    const void* w;
+    const void* b;
+    float* mean;       // [rows] written by the forward (or null), read by the backward
+    float* rstd;
+    float* part;       // backward: [blocks][2][width] partials of dw and db (or null)
+    int64_t rows, x_pitch, dy_pitch;
+    int32_t width;
+    int32_t w_f32;     // w and b are fp32 beside 16-bit x
+    float eps;
+};
+
+template <typename T>
+__device__ __forceinline__ float param_at(const void* p, int w_f32, int64_t c) {
+    return w_f32 ? ((const float*)p)[c] : (float)((const T*)p)[c];
+}
+
+// The sum of N values over the TPR threads of a row: a butterfly inside a wave, then LDS. `lds`
+// holds two buffers used in turn, so one barrier a sum is enough.
+template <int TPR, int N>
+__device__ __forceinline__ void row_sum(float (&v)[N], float* lds, int& turn) {
+    constexpr int LANES = TPR < 64 ? TPR : 64;
+#pragma unroll
+    for (int d = LANES / 2; d > 0; d >>= 1)
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], d, 64);
+    if constexpr (TPR > 64) {
+        constexpr int W = TPR / 64;
+        float* buf = lds + turn * (W * 2);
+        turn ^= 1;
+        if (threadIdx.x % 64 == 0) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) buf[(threadIdx.x / 64) * 2 + i] = v[i];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float s = buf[i];
+#pragma unroll
+            for (int w = 1; w < W; ++w) s += buf[w * 2 + i];
+            v[i] = s;
+        }
+    }
+}
+
+template <int TPR>
+struct RowShape {
+    static constexpr int threads = TPR > 256 ? TPR : 256;
+    static constexpr int rows = threads / TPR;          // rows a workgroup has at a time
+    static constexpr int lds = TPR > 64 ? TPR / 64 * 4 : 1;
+};
+
+template <typename T, int V, int TPR, int NV>
+__global__ __launch_bounds__(RowShape<TPR>::threads) void layer_norm_fwd_kernel(NormArgs a) {
+    using S = RowShape<TPR>;
+    __shared__ float lds[S::lds];
+    const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+    const int F = a.width;
+    float w[NV][V], b[NV][V];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int c = (i * TPR + t) * V + j;
+            w[i][j] = a.w && c < F ? param_at<T>(a.w, a.w_f32, c) : 1.0f;
+            b[i][j] = a.b && c < F ? param_at<T>(a.b, a.w_f32, c) : 0.0f;
+        }
+    const float width = (float)F;
+    int turn = 0;
+    const int64_t step = (int64_t)gridDim.x * S::rows;
+    // every thread of the workgroup takes part in each turn's sums; rows past the end are not touched
+    for (int64_t r0 = (int64_t)blockIdx.x * S::rows; r0 < a.rows; r0 += step) {
+        const int64_t r = r0 + sub;
+        const bool live = r < a.rows;
+        const T* x = (const T*)a.x + r * a.x_pitch;
+        float v[NV][V], s[1] = {0.0f};
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * TPR + t) * V;
+            if (live && c < F) {
+                load_vec<T, V>(v[i], x + c);
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; ++j) v[i][j] = 0.0f;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j) s[0] += v[i][j];
+        row_sum<TPR, 1>(s, lds, turn);
+        const float mean = s[0] / width;
+        float q[1] = {0.0f};
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const bool in = (i * TPR + t) * V < F;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                v[i][j] -= mean;
+                if (in) q[0] = __builtin_fmaf(v[i][j], v[i][j], q[0]);
+            }
+        }
+        row_sum<TPR, 1>(q, lds, turn);
+        const float rstd = 1.0f / sqrtf(q[0] / width + a.eps);
+        if (!live) continue;
+        T* y = (T*)a.out + r * F;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * TPR + t) * V;
+            if (c >= F) continue;
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[i][j] = __builtin_fmaf(v[i][j] * rstd, w[i][j], b[i][j]);
+            store_vec<T, V>(y + c, v[i]);
+        }
+        if (a.mean && t == 0) {
+            a.mean[r] = mean;
+            a.rstd[r] = rstd;
+        }
+    }
+}
+
+// a + v with the rounding error carried in c (Kahan's sum); plain for 16-bit inputs, whose outputs
+// round far coarser than the sum
+template <bool COMP>
+__device__ __forceinline__ void add_to(float& a, float& c, float v) {
+    if constexpr (COMP) {
+        const float u = v - c;
+        const float s = a + u;
+        c = (s - a) - u;
+        a = s;
+    } else {
+        a += v;
+    }
+}
+
+template <typename T, int V, int TPR, int NV>
+__global__ __launch_bounds__(RowShape<TPR>::threads) void layer_norm_bwd_kernel(NormArgs a) {
+    using S = RowShape<TPR>;
+    constexpr bool COMP = sizeof(T) == 4;
+    constexpr int COLS = TPR * NV * V;
+    __shared__ float lds[S::lds];
+    __shared__ float s_part[S::rows > 1 ? S::rows * COLS : 1];
+    const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+    const int F = a.width;
+    float w[NV][V], dw[NV][V], db[NV][V], dwc[COMP ? NV : 1][V], dbc[COMP ? NV : 1][V];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int c = (i * TPR + t) * V + j;
+            w[i][j] = a.w && c < F ? param_at<T>(a.w, a.w_f32, c) : 1.0f;
+            dw[i][j] = db[i][j] = 0.0f;
+            dwc[COMP ? i : 0][j] = dbc[COMP ? i : 0][j] = 0.0f;
+        }
+    const float width = (float)F;
+    int turn = 0;
+    const int64_t step = (int64_t)gridDim.x * S::rows;
+    for (int64_t r0 = (int64_t)blockIdx.x * S::rows; r0 < a.rows; r0 += step) {
+        const int64_t r = r0 + sub;
+        const bool live = r < a.rows;
+        const T* x = (const T*)a.x + r * a.x_pitch;
+        const T* dy = (const T*)a.dy + r * a.dy_pitch;
+        const float mean = live ? a.mean[r] : 0.0f, rstd = live ? a.rstd[r] : 0.0f;
+        float xh[NV][V], g[NV][V], s[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * TPR + t) * V;
+            if (live && c < F) {
+                load_vec<T, V>(xh[i], x + c);
+                load_vec<T, V>(g[i], dy + c);
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; ++j) xh[i][j] = g[i][j] = 0.0f;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const bool in = live && (i * TPR + t) * V < F;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                if (!in) continue;
+                xh[i][j] = (xh[i][j] - mean) * rstd;
+                add_to<COMP>(dw[i][j], dwc[COMP ? i : 0][j], g[i][j] * xh[i][j]);
+                add_to<COMP>(db[i][j], dbc[COMP ? i : 0][j], g[i][j]);
+                g[i][j] *= w[i][j];
+                s[0] += g[i][j];
+                s[1] = __builtin_fmaf(g[i][j], xh[i][j], s[1]);
+            }
+        }
+        if (!a.out) continue;
+        row_sum<TPR, 2>(s, lds, turn);
+        if (!live) continue;
+        const float m1 = s[0] / width, m2 = s[1] / width;
+        T* dx = (T*)a.out + r * F;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * TPR + t) * V;
+            if (c >= F) continue;
+#pragma unroll
+            for (int j = 0; j < V; ++j) g[i][j] = rstd * (g[i][j] - m1 - xh[i][j] * m2);
+            store_vec<T, V>(dx + c, g[i]);
+        }
+    }
+    if (!a.part) return;
+    // one partial row per workgroup: its row slots added in order through LDS
+    float* pw = a.part + (int64_t)blockIdx.x * 2 * F;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        float(&d)[NV][V] = k ? db : dw;
+        if constexpr (S::rows > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int j = 0; j < V; ++j) s_part[sub * COLS + (i * TPR + t) * V + j] = d[i][j];
+            __syncthreads();
+            for (int c = threadIdx.x; c < F; c += S::threads) {
+                float v = s_part[c];
+                for (int q = 1; q < S::rows; ++q) v += s_part[q * COLS + c];
+                pw[(int64_t)k * F + c] = v;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const int c = (i * TPR + t) * V + j;
+                    if (c < F) pw[(int64_t)k * F + c] = d[i][j];
+                }
+        }
+    }
+}
+
+// Rows too wide for registers: a workgroup per row, which is read again (from L2) for each sum.
+constexpr int kWide = 1024;
+
+template <typename T>
+__global__ __launch_bounds__(kWide) void layer_norm_fwd_wide_kernel(NormArgs a) {
+    __shared__ float lds[kWide / 64 * 4];
+    const int F = a.width;
+    int turn = 0;
+    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        const T* x = (const T*)a.x + r * a.x_pitch;
+        T* y = (T*)a.out + r * F;
+        float s[1] = {0.0f}, q[1] = {0.0f};
+        for (int c = threadIdx.x; c < F; c += kWide) s[0] += (float)x[c];
+        row_sum<kWide, 1>(s, lds, turn);
+        const float mean = s[0] / (float)F;
+        for (int c = threadIdx.x; c < F; c += kWide) {
+            const float d = (float)x[c] - mean;
+            q[0] = __builtin_fmaf(d, d, q[0]);
+        }
+        row_sum<kWide, 1>(q, lds, turn);
+        const float rstd = 1.0f / sqrtf(q[0] / (float)F + a.eps);
+        for (int c = threadIdx.x; c < F; c += kWide) {
+            const float w = a.w ? param_at<T>(a.w, a.w_f32, c) : 1.0f, b = a.b ? param_at<T>(a.b, a.w_f32, c) : 0.0f;
+            y[c] = (T)__builtin_fmaf(((float)x[c] - mean) * rstd, w, b);
+        }
+        if (a.mean && threadIdx.x == 0) {
+            a.mean[r] = mean;
+            a.rstd[r] = rstd;
+        }
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kWide) void layer_norm_bwd_wide_kernel(NormArgs a) {
+    __shared__ float lds[kWide / 64 * 4];
+    const int F = a.width;
+    int turn = 0;
+    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        const T* x = (const T*)a.x + r * a.x_pitch;
+        const T* dy = (const T*)a.dy + r * a.dy_pitch;
+        T* dx = (T*)a.out + r * F;
+        const float mean = a.mean[r], rstd = a.rstd[r];
+        float s[2] = {0.0f, 0.0f};
+        for (int c = threadIdx.x; c < F; c += kWide) {
+            const float h = (float)dy[c] * (a.w ? param_at<T>(a.w, a.w_f32, c) : 1.0f);
+            s[0] += h;
+            s[1] = __builtin_fmaf(h, ((float)x[c] - mean) * rstd, s[1]);
+        }
+        row_sum<kWide, 2>(s, lds, turn);
+        const float m1 = s[0] / (float)F, m2 = s[1] / (float)F;
+        for (int c = threadIdx.x; c < F; c += kWide) {
+            const float h = (float)dy[c] * (a.w ? param_at<T>(a.w, a.w_f32, c) : 1.0f);
+            dx[c] = (T)(rstd * (h - m1 - ((float)x[c] - mean) * rstd * m2));
+        }
+    }
+}
+
+// dw and db partials of wide rows: a thread per column, a row slice per blockIdx.y
+template <typename T>
+__global__ __launch_bounds__(256) void layer_norm_cols_kernel(NormArgs a, int64_t slice) {
+    const int c = blockIdx.x * 256 + threadIdx.x;
+    if (c >= a.width) return;
+    const int64_t lo = (int64_t)blockIdx.y * slice, hi = min(lo + slice, a.rows);
+    float dw = 0.0f, db = 0.0f, dwc = 0.0f, dbc = 0.0f;
+    for (int64_t r = lo; r < hi; ++r) {
+        const float g = (float)((const T*)a.dy)[r * a.dy_pitch + c];
+        const float xh = ((float)((const T*)a.x)[r * a.x_pitch + c] - a.mean[r]) * a.rstd[r];
+        add_to<true>(dw, dwc, g * xh);
+        add_to<true>(db, dbc, g);
+    }
+    float* p = a.part + (int64_t)blockIdx.y * 2 * a.width;
+    p[c] = dw;
+    p[(int64_t)a.width + c] = db;
+}
+
+// out[c] = sum over p of part[p][c], c over dw's columns then db's: 16 columns x 16 row slices a
+// workgroup, the slices joined in order
+template <typename T>
+__global__ __launch_bounds__(256) void layer_norm_reduce_kernel(const float* part, int n_part, int32_t width, T* dw,
+                                                                 T* db, float* dw32, float* db32) {
+    __shared__ double s[16][17];
+    const int64_t cols = 2 * (int64_t)width;
+    const int64_t c = (int64_t)blockIdx.x * 16 + threadIdx.x % 16;
+    const int slice = threadIdx.x / 16;
+    double v = 0.0;
+    if (c < cols) {
+#pragma unroll 4
+        for (int p = slice; p < n_part; p += 16) v += (double)part[(int64_t)p * cols + c];
+    }
+    s[slice][threadIdx.x % 16] = v;
+    __syncthreads();
+    if (slice || c >= cols) return;
+    for (int k = 1; k < 16; ++k) v += s[k][threadIdx.x % 16];
+    const int64_t col = c < width ? c : c - width;
+    T* o = c < width ? dw : db;
+    float* o32 = c < width ? dw32 : db32;
+    if (o) o[col] = (T)(float)v;
+    if (o32) o32[col] = (float)v;
+}
+
+constexpr int kNormPartials = 512;   // workgroups (and partial rows) of a backward
+
+template <typename T, int V, int TPR, int NV>
+void launch_rows(const NormArgs& a, bool bwd, int max_blocks, hipStream_t strm) {
+    using S = RowShape<TPR>;
+    const int blocks = (int)std::min<int64_t>(max_blocks, (a.rows + S::rows - 1) / S::rows);
+    if (bwd)
+        hipLaunchKernelGGL((layer_norm_bwd_kernel<T, V, TPR, NV>), dim3(blocks), dim3(S::threads), 0, strm, a);
+    else
+        hipLaunchKernelGGL((layer_norm_fwd_kernel<T, V, TPR, NV>), dim3(blocks), dim3(S::threads), 0, strm, a);
+}
+
+// The narrowest team of threads that holds a row of `vecs` vectors; false: none does.
+template <typename T, int V>
+bool launch_by_width(const NormArgs& a, bool bwd, int max_blocks, hipStream_t strm) {
+    const int vecs = (a.width + V - 1) / V;
+    if (vecs <= 16) launch_rows<T, V, 16, 1>(a, bwd, max_blocks, strm);
+    else if (vecs <= 32) launch_rows<T, V, 32, 1>(a, bwd, max_blocks, strm);
+    else if (vecs <= 64) launch_rows<T, V, 64, 1>(a, bwd, max_blocks, strm);
+    else if (vecs <= 128) launch_rows<T, V, 64, 2>(a, bwd, max_blocks, strm);
+    else if (vecs <= 256) launch_rows<T, V, 256, 1>(a, bwd, max_blocks, strm);
+    else if (vecs <= 512) launch_rows<T, V, 256, 2>(a, bwd, max_blocks, strm);
+    else if (vecs <= 1024) launch_rows<T, V, 256, 4>(a, bwd, max_blocks, strm);
+    else if (vecs <= 2048) launch_rows<T, V, 1024, 2>(a, bwd, max_blocks, strm);
+    else return false;
+    return true;
+}
+
+bool vec_ok(const NormArgs& a, int eb) {
+    const int v = 16 / eb;
+    return a.width % v == 0 && a.x_pitch % v == 0 && a.dy_pitch % v == 0 && aligned16(a.x) && aligned16(a.dy) &&
+           aligned16(a.out);
+}
+
+int64_t norm_partials(int64_t rows) { return std::min<int64_t>(rows, kNormPartials); }
+
+template <typename T>
+int32_t norm_fwd(const NormArgs& a, hipStream_t strm) {
+    constexpr int max_blocks = 256 * 16;
+    const bool done = vec_ok(a, sizeof(T)) ? launch_by_width<T, 16 / sizeof(T)>(a, false, max_blocks, strm)
+                                           : launch_by_width<T, 1>(a, false, max_blocks, strm);
+    if (!done)
+        hipLaunchKernelGGL(layer_norm_fwd_wide_kernel<T>, dim3((unsigned)std::min<int64_t>(a.rows, 1024)), dim3(kWide),
+                           0, strm, a);
+    return launch_status("mpgnn_layer_norm_fwd: the launch failed");
+}
+
+template <typename T>
+int32_t norm_bwd(const NormArgs& a, void* dw, void* db, hipStream_t strm) {
+    int parts = 0;
+    const int V = vec_ok(a, sizeof(T)) ? 16 / (int)sizeof(T) : 1;
+    const int vecs = (a.width + V - 1) / V;
+    const int rows_per = vecs <= 16 ? 16 : vecs <= 32 ? 8 : vecs <= 128 ? 4 : 1;
+    if (a.rows == 0) {  // no partial rows: the parameters' gradients are zero
+    } else if (vecs <= 2048) {
+        parts = (int)std::min<int64_t>(kNormPartials, (a.rows + rows_per - 1) / rows_per);
+        if (V == 1) launch_by_width<T, 1>(a, true, kNormPartials, strm);
+        else launch_by_width<T, 16 / sizeof(T)>(a, true, kNormPartials, strm);
+    } else {
+        if (a.out)
+            hipLaunchKernelGGL(layer_norm_bwd_wide_kernel<T>, dim3((unsigned)std::min<int64_t>(a.rows, 1024)),
+                               dim3(kWide), 0, strm, a);
+        if (a.part) {
+            const int64_t slice = (a.rows + kNormPartials - 1) / kNormPartials;
+            parts = (int)((a.rows + slice - 1) / slice);
+            hipLaunchKernelGGL(layer_norm_cols_kernel<T>, dim3((a.width + 255) / 256, parts), dim3(256), 0, strm, a,
+                               slice);
+        }
+    }
+    if (a.part) {
+        T* w = a.w_f32 ? nullptr : (T*)dw;
+        T* b = a.w_f32 ? nullptr : (T*)db;
+        float* w32 = a.w_f32 ? (float*)dw : nullptr;
+        float* b32 = a.w_f32 ? (float*)db : nullptr;
+        hipLaunchKernelGGL(layer_norm_reduce_kernel<T>, dim3((unsigned)((2 * (int64_t)a.width + 15) / 16)), dim3(256), 0,
+                           strm, a.part, parts, a.width, w, b, w32, b32);
+    }
+    return launch_status("mpgnn_layer_norm_bwd: a launch failed");
+}
+
+int32_t check_norm(int64_t rows, int64_t width, int64_t pitch, int32_t dtype, int32_t wdtype) {
+    if (rows < 0 || width <= 0 || (rows > 1 && pitch < width))
+        return arg_error("layer norm: rows < 0, width < 1 or a row pitch below the width");
+    if (!dtype_bytes(dtype)) return arg_error("layer norm: unknown dtype");
+    if (wdtype != dtype && wdtype != MPGNN_F32)
+        return arg_error("layer norm: weight and bias must have the input's type or fp32");
+    if (width > (1 << 24)) return unsupported("layer norm: more than 2^24 columns");
+    return MPGNN_OK;
+}
+
+}  // namespace
+}  // namespace mpgnn
+
+extern "C" int32_t mpgnn_layer_norm_fwd(const void* x, int64_t rows, int64_t width, int64_t x_pitch, int32_t dtype,
+                                        const void* weight, const void* bias, int32_t wdtype, double eps, void* y,
+                                        float* mean, float* rstd, void* stream) {
+    using namespace mpgnn;
+    int32_t st = check_norm(rows, width, x_pitch, dtype, wdtype);
+    if (st != MPGNN_OK) return st;
+    if (rows == 0) return MPGNN_OK;
+    if (!x || !y || (mean == nullptr) != (rstd == nullptr))
+        return arg_error("mpgnn_layer_norm_fwd: x or y is null, or one of mean and rstd alone");
+    NormArgs a{};
+    a.x = x; a.out = y; a.w = weight; a.b = bias; a.mean = mean; a.rstd = rstd;
+    a.rows = rows; a.x_pitch = x_pitch; a.width = (int32_t)width; a.w_f32 = wdtype == MPGNN_F32; a.eps = (float)eps;
+    hipStream_t strm = static_cast<hipStream_t>(stream);
+    if (dtype == MPGNN_F32) return norm_fwd<float>(a, strm);
+    return dtype == MPGNN_BF16 ? norm_fwd<__bf16>(a, strm) : norm_fwd<_Float16>(a, strm);
+}
+
+extern "C" int32_t mpgnn_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t width, int64_t* bytes) {
+    using namespace mpgnn;
+    if (rows < 0 || width <= 0 || !bytes)
+        return arg_error("mpgnn_layer_norm_bwd_workspace_bytes: bad shape or bytes is null");
+    *bytes = norm_partials(rows) * 2 * width * (int64_t)sizeof(float);
+    return MPGNN_OK;
+}
+
+extern "C" int32_t mpgnn_layer_norm_bwd(const void* dy, int64_t dy_pitch, const void* x, int64_t x_pitch, int64_t rows,
+                                        int64_t width, int32_t dtype, const void* weight, int32_t wdtype,
+                                        const float* mean, const float* rstd, void* dx, void* dweight, void* dbias,
+                                        void* workspace, void* stream) {
+    using namespace mpgnn;
+    int32_t st = check_norm(rows, width, x_pitch, dtype, wdtype);
+    if (st != MPGNN_OK) return st;
+    if (rows > 1 && dy_pitch < width) return arg_error("mpgnn_layer_norm_bwd: dy's row pitch is below the width");
+    if ((dweight || dbias) && !workspace) return arg_error("mpgnn_layer_norm_bwd: no workspace");
+    if (rows > 0 && (!x || !dy || !mean || !rstd)) return arg_error("mpgnn_layer_norm_bwd: a null input");
+    if (!dx && !dweight && !dbias) return MPGNN_OK;
+    NormArgs a{};
+    a.x = x; a.dy = dy; a.out = dx; a.w = weight;
+    a.mean = const_cast<float*>(mean); a.rstd = const_cast<float*>(rstd);
+    a.part = dweight || dbias ? static_cast<float*>(workspace) : nullptr;
+    a.rows = rows; a.x_pitch = x_pitch; a.dy_pitch = dy_pitch; a.width = (int32_t)width; a.w_f32 = wdtype == MPGNN_F32;
+    hipStream_t strm = static_cast<hipStream_t>(stream);
+    if (dtype == MPGNN_F32) return norm_bwd<float>(a, dweight, dbias, strm);
+    return dtype == MPGNN_BF16 ? norm_bwd<__bf16>(a, dweight, dbias, strm) : norm_bwd<_Float16>(a, dweight, dbias, strm);
+}

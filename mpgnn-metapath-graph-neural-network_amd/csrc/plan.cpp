@@ -37,6 +37,13 @@ static thread_local std::string g_last_error;
 
 void set_last_error(const std::string& msg) { g_last_error = msg; }
 
+void set_last_error_cstr(const char* msg) noexcept {
+    try {
+        g_last_error = msg;
+    } catch (...) {  // out of memory: the status alone tells
+    }
+}
+
 static int32_t fail(int32_t code, const std::string& msg) {
     set_last_error(msg);
     return code;

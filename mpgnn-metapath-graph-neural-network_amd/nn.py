@@ -16,9 +16,10 @@ from torch.nn import Parameter
 
 from .functional import MODE_ALL, rgcn_conv
 from .mp_rgcn_layer import glorot, zeros
+from .operators import grouped_linear, layer_norm
 from .plan import FLOWS, get_plan
 
-__all__ = ["RGCNConv", "FastRGCNConv", "CustomFastRGCNConv"]
+__all__ = ["RGCNConv", "FastRGCNConv", "CustomFastRGCNConv", "LayerNorm", "GroupedLinear"]
 
 
 class RGCNConv(torch.nn.Module):
@@ -133,3 +134,71 @@ class FastRGCNConv(RGCNConv):
 
 
 CustomFastRGCNConv = FastRGCNConv
+
+
+class LayerNorm(torch.nn.Module):
+    """``torch.nn.LayerNorm(normalized_shape)`` over the last dimension (same parameters, names and
+    initialisation; a shape of more than one dimension is not supported) on ``operators.layer_norm``."""
+
+    def __init__(self, normalized_shape, eps: float = 1e-5, elementwise_affine: bool = True, bias: bool = True,
+                 device=None, dtype=None):
+        super().__init__()
+        shape = (normalized_shape,) if isinstance(normalized_shape, int) else tuple(normalized_shape)
+        if len(shape) != 1:
+            raise NotImplementedError(f"normalisation over {len(shape)} dimensions (the last one only)")
+        self.normalized_shape = shape
+        self.eps = eps
+        self.elementwise_affine = elementwise_affine
+        if elementwise_affine:
+            self.weight = Parameter(torch.ones(shape, device=device, dtype=dtype))
+        else:
+            self.register_parameter("weight", None)
+        if elementwise_affine and bias:
+            self.bias = Parameter(torch.zeros(shape, device=device, dtype=dtype))
+        else:
+            self.register_parameter("bias", None)
+
+    def reset_parameters(self):
+        with torch.no_grad():
+            if self.weight is not None:
+                self.weight.fill_(1.0)
+        zeros(self.bias)
+
+    def forward(self, x: Tensor) -> Tensor:
+        if x.dim() == 0 or x.shape[-1] != self.normalized_shape[0]:
+            raise RuntimeError(f"Given normalized_shape={list(self.normalized_shape)}, expected input with last "
+                               f"dimension {self.normalized_shape[0]}, but got input of size {list(x.shape)}")
+        return layer_norm(x, self.weight, self.bias, self.eps)
+
+    def extra_repr(self) -> str:
+        return f"{self.normalized_shape}, eps={self.eps}, elementwise_affine={self.elementwise_affine}"
+
+
+class GroupedLinear(torch.nn.Module):
+    """A linear layer with a weight per group (node type, relation, expert) over rows sorted by group:
+    ``operators.grouped_linear`` with ``weight`` [groups, in, out] and ``bias`` [groups, out], initialised as
+    RGCNConv's are (glorot, zeros). ``forward(x, group_ptr)``: group g owns rows group_ptr[g] to
+    group_ptr[g + 1] of x."""
+
+    def __init__(self, in_channels: int, out_channels: int, num_groups: int, bias: bool = True, device=None,
+                 dtype=None):
+        super().__init__()
+        self.in_channels = in_channels
+        self.out_channels = out_channels
+        self.num_groups = num_groups
+        self.weight = Parameter(torch.empty(num_groups, in_channels, out_channels, device=device, dtype=dtype))
+        if bias:
+            self.bias = Parameter(torch.empty(num_groups, out_channels, device=device, dtype=dtype))
+        else:
+            self.register_parameter("bias", None)
+        self.reset_parameters()
+
+    def reset_parameters(self):
+        glorot(self.weight)
+        zeros(self.bias)
+
+    def forward(self, x: Tensor, group_ptr: Tensor) -> Tensor:
+        return grouped_linear(x, self.weight, group_ptr, self.bias)
+
+    def extra_repr(self) -> str:
+        return f"{self.in_channels}, {self.out_channels}, num_groups={self.num_groups}"

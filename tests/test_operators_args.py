@@ -1,0 +1,117 @@
+"""CPU: layer_norm, grouped_linear and the clipping refuse CPU tensors and bad arguments before any
+launch, and size their workspaces on the host."""
+import ctypes
+
+import pytest
+import torch
+
+import mpgnn_amd
+from mpgnn_amd import _lib
+from mpgnn_amd._lib import lib
+
+P = ctypes.c_void_p(4096)
+
+
+def test_cpu_tensors_are_refused():
+    x, w = torch.zeros(4, 8), torch.zeros(2, 8, 5)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        mpgnn_amd.layer_norm(x)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        mpgnn_amd.grouped_linear(x, w, torch.tensor([0, 2, 4]))
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        mpgnn_amd.clip_by_global_norm([x], 1.0)
+    p = torch.nn.Parameter(x)
+    p.grad = torch.ones_like(x)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        mpgnn_amd.clip_grad_norm_([p], 1.0)
+    assert torch.equal(p.grad, torch.ones_like(x))
+    assert float(mpgnn_amd.clip_grad_norm_([torch.nn.Parameter(x)], 1.0)) == 0.0
+
+
+def test_layer_norm_entry_points_check_their_arguments():
+    def fwd(x=P, rows=4, width=8, pitch=8, dt=0, wdt=0, y=P, mean=None, rstd=None):
+        return lib.mpgnn_layer_norm_fwd(x, rows, width, pitch, dt, None, None, wdt, 1e-5, y, mean, rstd, None)
+
+    assert fwd(rows=0, x=None, y=None) == _lib.MPGNN_OK
+    for kw in (dict(rows=-1), dict(width=0), dict(pitch=7), dict(dt=3), dict(dt=0, wdt=1), dict(x=None), dict(y=None),
+               dict(mean=P)):
+        assert fwd(**kw) == _lib.MPGNN_ERR_ARG, kw
+    assert fwd(width=1 << 25, pitch=1 << 25) == _lib.MPGNN_ERR_UNSUPPORTED
+
+    def bwd(dy=P, dpitch=8, rows=4, stats=P, dx=P, dw=None, ws=None):
+        return lib.mpgnn_layer_norm_bwd(dy, dpitch, P, 8, rows, 8, 0, None, 0, stats, stats, dx, dw, None, ws, None)
+
+    assert bwd(dx=None) == _lib.MPGNN_OK  # nothing wanted
+    for kw in (dict(dy=None), dict(dpitch=5), dict(rows=-2), dict(stats=None), dict(dw=P)):
+        assert bwd(**kw) == _lib.MPGNN_ERR_ARG, kw
+    nb = ctypes.c_int64()
+    assert lib.mpgnn_layer_norm_bwd_workspace_bytes(10, 16, ctypes.byref(nb)) == 0 and nb.value == 10 * 2 * 16 * 4
+    assert lib.mpgnn_layer_norm_bwd_workspace_bytes(10, 0, ctypes.byref(nb)) == _lib.MPGNN_ERR_ARG
+
+
+def test_grouped_linear_entry_points_check_their_arguments():
+    def fwd(x=P, rows=4, pitch=8, dt=0, w=P, groups=2, k=8, n=5, ptr=P, bits=64, out=P):
+        return lib.mpgnn_grouped_linear_fwd(x, rows, pitch, dt, w, groups, k, n, None, ptr, bits, out, None)
+
+    def dgrad(dy=P, rows=4, pitch=5, dt=0, w=P, groups=2, k=8, n=5, ptr=P, bits=64, out=P):
+        return lib.mpgnn_grouped_linear_dgrad(dy, rows, pitch, dt, w, groups, k, n, ptr, bits, out, None)
+
+    for f in (fwd, dgrad):
+        assert f(rows=0) == _lib.MPGNN_OK
+        for kw in (dict(rows=-1), dict(pitch=4), dict(dt=9), dict(w=None), dict(groups=0), dict(k=0), dict(n=0),
+                   dict(ptr=None), dict(bits=16), dict(out=None)):
+            assert f(**kw) == _lib.MPGNN_ERR_ARG, kw
+        assert f(k=1 << 25, n=1 << 25, pitch=1 << 26) == _lib.MPGNN_ERR_UNSUPPORTED
+    assert fwd(x=None) == _lib.MPGNN_ERR_ARG
+
+    def wgrad(rows=4, xp=8, dp=5, dw=P, ws=None, groups=2, k=8, n=5):
+        return lib.mpgnn_grouped_linear_wgrad(P, xp, P, dp, rows, 0, groups, k, n, P, 64, dw, None, ws, None)
+
+    for kw in (dict(rows=-1), dict(xp=7), dict(dp=4), dict(dw=None), dict(rows=1 << 20)):  # the last: no workspace
+        assert wgrad(**kw) == _lib.MPGNN_ERR_ARG, kw
+    nb = ctypes.c_int64()
+    # a weight with tiles enough to fill the chip needs none; one tile over many rows does
+    assert lib.mpgnn_grouped_linear_wgrad_workspace_bytes(1 << 15, 32, 2048, 4096, ctypes.byref(nb)) == 0
+    assert nb.value == 0
+    assert lib.mpgnn_grouped_linear_wgrad_workspace_bytes(1 << 20, 2, 128, 128, ctypes.byref(nb)) == 0
+    assert nb.value >= 2 * 128 * 128 * 4
+    assert lib.mpgnn_grouped_linear_wgrad_workspace_bytes(4, 2, 8, 5, None) == _lib.MPGNN_ERR_ARG
+
+
+def test_clip_entry_point_checks_its_arguments():
+    arr = (_lib.ClipTensor * 2)()
+    for t in arr:
+        t.grad, t.out, t.numel, t.dtype = 4096, 8192, 16, _lib.F32
+
+    def clip(n=2, kind=_lib.NORM_2, norm=P, ws=P):
+        return lib.mpgnn_clip_by_global_norm(ctypes.addressof(arr), n, kind, 1.0, norm, ws, None)
+
+    assert clip(n=0) == clip(n=-1) == clip(kind=1) == clip(norm=None) == clip(ws=None) == _lib.MPGNN_ERR_ARG
+    assert lib.mpgnn_clip_by_global_norm(None, 1, 2, 1.0, P, P, None) == _lib.MPGNN_ERR_ARG
+    for k in range(2):  # out for one tensor only
+        arr[k].out = None
+        assert clip() == _lib.MPGNN_ERR_ARG
+        arr[k].out = 8192
+    for field, v, back in (("dtype", 7, 0), ("numel", -1, 16), ("grad", None, 4096), ("grad", 4098, 4096),
+                           ("out", 8193, 8192)):
+        setattr(arr[1], field, v)
+        assert clip() == _lib.MPGNN_ERR_ARG, field
+        setattr(arr[1], field, back)
+    arr[0].numel = 1 << 41
+    assert clip() == _lib.MPGNN_ERR_UNSUPPORTED
+    nb = ctypes.c_int64()
+    assert lib.mpgnn_clip_workspace_bytes(3, ctypes.byref(nb)) == 0 and nb.value == 2048 * 8
+    assert lib.mpgnn_clip_workspace_bytes(-3, ctypes.byref(nb)) == _lib.MPGNN_ERR_ARG
+
+
+def test_modules_match_torch_parameters():
+    a, b = mpgnn_amd.LayerNorm(12), torch.nn.LayerNorm(12)
+    assert a.state_dict().keys() == b.state_dict().keys()
+    assert all(torch.equal(x, y) for x, y in zip(a.state_dict().values(), b.state_dict().values()))
+    assert mpgnn_amd.LayerNorm(12, elementwise_affine=False).weight is None
+    assert mpgnn_amd.LayerNorm(12, bias=False).bias is None
+    with pytest.raises(NotImplementedError):
+        mpgnn_amd.LayerNorm((3, 4))
+    g = mpgnn_amd.GroupedLinear(6, 4, 3)
+    assert tuple(g.weight.shape) == (3, 6, 4) and tuple(g.bias.shape) == (3, 4) and float(g.bias.abs().max()) == 0.0
+    assert float(g.weight.abs().max()) <= (6.0 / (6 + 4)) ** 0.5
