@@ -184,24 +184,34 @@ __device__ __forceinline__ Raw<T> load8(const T* p, int valid) {
     return r;
 }
 
+__device__ __forceinline__ unsigned pack_bf16(float a, float b) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2{a, b}), bf16x2));
+}
+
 template <typename T>
 __device__ __forceinline__ void store8(typename Stage<T>::elem* dst, int plane_size, const Raw<T>& r) {
     if constexpr (sizeof(T) == 2) {
         *reinterpret_cast<u32x4*>(dst) = r.v[0];
     } else {
+        // by pairs: one conversion instruction a piece, and the pieces stay packed
         float f[8];
         __builtin_memcpy(f, &r, sizeof(f));
-        bf16x8 p0, p1, p2;
+        u32x4 p0, p1, p2;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            p0[i] = (__bf16)f[i];
-            const float d = f[i] - (float)p0[i];
-            p1[i] = (__bf16)d;
-            p2[i] = (__bf16)(d - (float)p1[i]);
+        for (int i = 0; i < 4; ++i) {
+            const unsigned u0 = pack_bf16(f[2 * i], f[2 * i + 1]);
+            const float a = f[2 * i] - __uint_as_float(u0 << 16);
+            const float b = f[2 * i + 1] - __uint_as_float(u0 & 0xffff0000u);
+            const unsigned u1 = pack_bf16(a, b);
+            p0[i] = u0;
+            p1[i] = u1;
+            p2[i] = pack_bf16(a - __uint_as_float(u1 << 16), b - __uint_as_float(u1 & 0xffff0000u));
         }
-        *reinterpret_cast<bf16x8*>(dst) = p0;
-        *reinterpret_cast<bf16x8*>(dst + plane_size) = p1;
-        *reinterpret_cast<bf16x8*>(dst + 2 * plane_size) = p2;
+        *reinterpret_cast<u32x4*>(dst) = p0;
+        *reinterpret_cast<u32x4*>(dst + plane_size) = p1;
+        *reinterpret_cast<u32x4*>(dst + 2 * plane_size) = p2;
     }
 }
 

@@ -1648,6 +1648,29 @@ __device__ __forceinline__ void split3_bf16(float a, __bf16& h0, __bf16& h1, __b
     h2 = (__bf16)r2;
 }
 
+// split3_bf16 of two neighbours at once, on packed pairs: one conversion instruction per piece and
+// pair, and the pieces stay in packed registers (element by element, without packed fp32
+// subtraction, the compiler converts each half on its own and the weight slices spill)
+__device__ __forceinline__ void split3_bf16x2(float a, float b, __bf16* h0, __bf16* h1, __bf16* h2) {
+#ifdef MPGNN_PROBE_NOSPLIT
+    split3_bf16(a, h0[0], h1[0], h2[0]);
+    split3_bf16(b, h0[1], h1[1], h2[1]);
+    return;
+#endif
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const bf16x2 p0 = __builtin_convertvector((f32x2{a, b}), bf16x2);
+    const unsigned u0 = __builtin_bit_cast(unsigned, p0);
+    const float ra = a - __uint_as_float(u0 << 16), rb = b - __uint_as_float(u0 & 0xffff0000u);
+    const bf16x2 p1 = __builtin_convertvector((f32x2{ra, rb}), bf16x2);
+    const unsigned u1 = __builtin_bit_cast(unsigned, p1);
+    const bf16x2 p2 = __builtin_convertvector(
+        (f32x2{ra - __uint_as_float(u1 << 16), rb - __uint_as_float(u1 & 0xffff0000u)}), bf16x2);
+    h0[0] = p0[0]; h0[1] = p0[1];
+    h1[0] = p1[0]; h1[1] = p1[1];
+    h2[0] = p2[0]; h2[1] = p2[1];
+}
+
 template <int KB, bool DGRAD>
 struct RelGemmBf3 {
     using Base = RelGemm<KB, DGRAD>;
@@ -1671,10 +1694,8 @@ struct RelGemmBf3 {
             const int r = e / W4;
             const float4 x = r < it.nrows ? v[j] : make_float4(0.f, 0.f, 0.f, 0.f);
             __bf16 p0[4], p1[4], p2[4];
-            split3_bf16(x.x, p0[0], p1[0], p2[0]);
-            split3_bf16(x.y, p0[1], p1[1], p2[1]);
-            split3_bf16(x.z, p0[2], p1[2], p2[2]);
-            split3_bf16(x.w, p0[3], p1[3], p2[3]);
+            split3_bf16x2(x.x, x.y, p0, p1, p2);
+            split3_bf16x2(x.z, x.w, p0 + 2, p1 + 2, p2 + 2);
             __bf16* d = A + r * LDAB + (e % W4) * 4;
             typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
             *reinterpret_cast<bf16x4*>(d) = bf16x4{p0[0], p0[1], p0[2], p0[3]};
@@ -1708,12 +1729,12 @@ struct RelGemmBf3 {
 #pragma unroll
         for (int s = 0; s < NS; ++s)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                __bf16 h0, h1, h2;
-                split3_bf16(f[s][j], h0, h1, h2);
-                b[s][0][j] = h0;
-                b[s][1][j] = h1;
-                b[s][2][j] = h2;
+            for (int j = 0; j < 8; j += 2) {
+                __bf16 h0[2], h1[2], h2[2];
+                split3_bf16x2(f[s][j], f[s][j + 1], h0, h1, h2);
+                b[s][0][j] = h0[0]; b[s][0][j + 1] = h0[1];
+                b[s][1][j] = h1[0]; b[s][1][j + 1] = h1[1];
+                b[s][2][j] = h2[0]; b[s][2][j + 1] = h2[1];
             }
     }
     __device__ static __forceinline__ void load_b(const float* w, int wave, int lane, bf16x8 (&b)[NS][3]) {
@@ -1730,10 +1751,8 @@ struct RelGemmBf3 {
         const int r = e / W4;
         const float4 x = r < nrows ? v : make_float4(0.f, 0.f, 0.f, 0.f);
         __bf16 p0[4], p1[4], p2[4];
-        split3_bf16(x.x, p0[0], p1[0], p2[0]);
-        split3_bf16(x.y, p0[1], p1[1], p2[1]);
-        split3_bf16(x.z, p0[2], p1[2], p2[2]);
-        split3_bf16(x.w, p0[3], p1[3], p2[3]);
+        split3_bf16x2(x.x, x.y, p0, p1, p2);
+        split3_bf16x2(x.z, x.w, p0 + 2, p1 + 2, p2 + 2);
         __bf16* d = A + r * LDAB + (e % W4) * 4;
         typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
         *reinterpret_cast<bf16x4*>(d) = bf16x4{p0[0], p0[1], p0[2], p0[3]};
@@ -2140,10 +2159,8 @@ struct RelGemmW1 {
         const int r = (tid >> 5) + 8 * j;
         const float4 x = r < nrows ? v : make_float4(0.f, 0.f, 0.f, 0.f);
         __bf16 p0[4], p1[4], p2[4];
-        split3_bf16(x.x, p0[0], p1[0], p2[0]);
-        split3_bf16(x.y, p0[1], p1[1], p2[1]);
-        split3_bf16(x.z, p0[2], p1[2], p2[2]);
-        split3_bf16(x.w, p0[3], p1[3], p2[3]);
+        split3_bf16x2(x.x, x.y, p0, p1, p2);
+        split3_bf16x2(x.z, x.w, p0 + 2, p1 + 2, p2 + 2);
         __bf16* d = A + r * LDAB + (tid & 31) * 4;
         typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
         *reinterpret_cast<bf16x4*>(d) = bf16x4{p0[0], p0[1], p0[2], p0[3]};
@@ -2472,10 +2489,8 @@ struct SingleBf3 {
             const int r = e / W4;
             const float4 xv = it * 32 + r < a.N ? q.v[j] : make_float4(0.f, 0.f, 0.f, 0.f);
             __bf16 p0[4], p1[4], p2[4];
-            split3_bf16(xv.x, p0[0], p1[0], p2[0]);
-            split3_bf16(xv.y, p0[1], p1[1], p2[1]);
-            split3_bf16(xv.z, p0[2], p1[2], p2[2]);
-            split3_bf16(xv.w, p0[3], p1[3], p2[3]);
+            split3_bf16x2(xv.x, xv.y, p0, p1, p2);
+            split3_bf16x2(xv.z, xv.w, p0 + 2, p1 + 2, p2 + 2);
             __bf16* d = P + r * LDAB + (e % W4) * 4;
             typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
             *reinterpret_cast<bf16x4*>(d) = bf16x4{p0[0], p0[1], p0[2], p0[3]};
@@ -2683,10 +2698,8 @@ struct RelGemmBf3W {
             const int r = t / 32 + 8 * j;
             const float4 x = r < it.nrows ? v[j] : make_float4(0.f, 0.f, 0.f, 0.f);
             __bf16 p0[4], p1[4], p2[4];
-            split3_bf16(x.x, p0[0], p1[0], p2[0]);
-            split3_bf16(x.y, p0[1], p1[1], p2[1]);
-            split3_bf16(x.z, p0[2], p1[2], p2[2]);
-            split3_bf16(x.w, p0[3], p1[3], p2[3]);
+            split3_bf16x2(x.x, x.y, p0, p1, p2);
+            split3_bf16x2(x.z, x.w, p0 + 2, p1 + 2, p2 + 2);
             __bf16* d = P + r * LDAB + (t & 31) * 4;
             typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
             *reinterpret_cast<bf16x4*>(d) = bf16x4{p0[0], p0[1], p0[2], p0[3]};
@@ -2700,10 +2713,8 @@ struct RelGemmBf3W {
         const int r = t / 32 + 8 * j;
         const float4 x = r < nrows ? v : make_float4(0.f, 0.f, 0.f, 0.f);
         __bf16 p0[4], p1[4], p2[4];
-        split3_bf16(x.x, p0[0], p1[0], p2[0]);
-        split3_bf16(x.y, p0[1], p1[1], p2[1]);
-        split3_bf16(x.z, p0[2], p1[2], p2[2]);
-        split3_bf16(x.w, p0[3], p1[3], p2[3]);
+        split3_bf16x2(x.x, x.y, p0, p1, p2);
+        split3_bf16x2(x.z, x.w, p0 + 2, p1 + 2, p2 + 2);
         __bf16* d = P + r * LDAB + (t & 31) * 4;
         typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
         *reinterpret_cast<bf16x4*>(d) = bf16x4{p0[0], p0[1], p0[2], p0[3]};
@@ -2743,12 +2754,12 @@ struct RelGemmBf3W {
 #pragma unroll
         for (int s = 0; s < NS; ++s)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                __bf16 h0, h1, h2;
-                split3_bf16(f[s][j], h0, h1, h2);
-                b[s][0][j] = h0;
-                b[s][1][j] = h1;
-                b[s][2][j] = h2;
+            for (int j = 0; j < 8; j += 2) {
+                __bf16 h0[2], h1[2], h2[2];
+                split3_bf16x2(f[s][j], f[s][j + 1], h0, h1, h2);
+                b[s][0][j] = h0[0]; b[s][0][j + 1] = h0[1];
+                b[s][1][j] = h1[0]; b[s][1][j + 1] = h1[1];
+                b[s][2][j] = h2[0]; b[s][2][j + 1] = h2[1];
             }
     }
 };
@@ -4963,10 +4974,8 @@ __device__ __forceinline__ void bw_dgrad_half(const BwdArgs& A, int i_beg, int i
             const int r = e / W4, c4 = (e % W4) * 4;
             const float4 xv = r < cur.nrows ? vc[j] : make_float4(0.f, 0.f, 0.f, 0.f);
             __bf16 p0[4], p1[4], p2[4];
-            split3_bf16(xv.x, p0[0], p1[0], p2[0]);
-            split3_bf16(xv.y, p0[1], p1[1], p2[1]);
-            split3_bf16(xv.z, p0[2], p1[2], p2[2]);
-            split3_bf16(xv.w, p0[3], p1[3], p2[3]);
+            split3_bf16x2(xv.x, xv.y, p0, p1, p2);
+            split3_bf16x2(xv.z, xv.w, p0 + 2, p1 + 2, p2 + 2);
             typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
             __bf16* d = Rp + r * kBwLdab + c4;
             *reinterpret_cast<bf16x4*>(d) = bf16x4{p0[0], p0[1], p0[2], p0[3]};
