@@ -115,13 +115,14 @@ struct Item {
 
 // Item `id` of the list of all groups' parts: each group has ceil(rows / size) of them, at least
 // `least`. With `rest`, the rows before ptr[0] and from ptr[G] on follow as two more groups.
+template <int THREADS>
 __device__ __forceinline__ Item find_item(const GroupedArgs& a, int64_t id, int size, int least, bool rest) {
-    __shared__ int64_t s_wave[kGlThreads / 64];
+    __shared__ int64_t s_wave[THREADS / 64];
     __shared__ Item s_item;
     const int n = a.groups + (rest ? 2 : 0);
     if (threadIdx.x == 0) s_item.group = -1;
     int64_t base = 0;
-    for (int g0 = 0; g0 < n; g0 += kGlThreads) {
+    for (int g0 = 0; g0 < n; g0 += THREADS) {
         const int g = g0 + threadIdx.x;
         int64_t lo = 0, hi = 0, parts = 0;
         if (g < a.groups) {
@@ -147,7 +148,7 @@ __device__ __forceinline__ Item find_item(const GroupedArgs& a, int64_t id, int 
         if (threadIdx.x % 64 == 63) s_wave[threadIdx.x / 64] = sum;
         __syncthreads();
         int64_t before = base;
-        for (int w = 0; w < kGlThreads / 64; ++w) {
+        for (int w = 0; w < THREADS / 64; ++w) {
             if (w < (int)(threadIdx.x / 64)) before += s_wave[w];
             base += s_wave[w];
         }
@@ -215,18 +216,18 @@ __device__ __forceinline__ void store8(typename Stage<T>::elem* dst, int plane_s
     }
 }
 
-// A tile of IDX indices x BK of c.
-template <typename T, Layout L, int IDX>
+// A tile of IDX indices x BK of c, staged by THREADS threads.
+template <typename T, Layout L, int IDX, int THREADS>
 struct Tile {
     typedef typename Stage<T>::elem E;
     static constexpr int BK = Stage<T>::bk;
-    static constexpr int plane = IDX * BK;                         // elements
-    static constexpr int chunks = IDX * BK / 8 / kGlThreads;       // 8-element pieces per thread
-    static_assert(chunks >= 1, "every thread stages a piece");
+    static constexpr int plane = IDX * BK;                      // elements
+    static constexpr int chunks = IDX * BK / 8 / THREADS;       // 8-element pieces per thread
+    static_assert(chunks >= 1 && chunks * THREADS * 8 == plane, "the threads' pieces make up the tile");
 
     // piece n of a thread: (index, c) of its first element
-    static __device__ __forceinline__ void place(int n, int& idx, int& c) {
-        const int id = threadIdx.x + n * kGlThreads;
+    static __device__ __forceinline__ void place(int tid, int n, int& idx, int& c) {
+        const int id = tid + n * THREADS;
         if constexpr (L == ALONG) {
             idx = id / (BK / 8);
             c = id % (BK / 8) * 8;
@@ -235,14 +236,11 @@ struct Tile {
             idx = id % (IDX / 8) * 8;
         }
     }
+    static constexpr int swap = IDX / 16 < 8 ? IDX / 16 - 1 : 7;  // ACROSS: bits of c that move a 32-byte block
+    static __device__ __forceinline__ int turn(int idx) { return BK == 64 ? idx & 7 : (idx >> 1) & 3; }  // ALONG
     static __device__ __forceinline__ int offset(int idx, int c) {
-        if constexpr (L == ALONG) {
-            const int q = BK == 64 ? (c / 8) ^ (idx & 7) : (c / 8) ^ ((idx >> 1) & 3);
-            return idx * BK + q * 8 + c % 8;
-        } else {
-            constexpr int m = IDX / 16 < 8 ? IDX / 16 - 1 : 7;
-            return c * IDX + ((idx / 16) ^ (c & m)) * 16 + idx % 16;
-        }
+        if constexpr (L == ALONG) return idx * BK + ((c / 8) ^ turn(idx)) * 8 + c % 8;
+        else return c * IDX + ((idx / 16) ^ (c & swap)) * 16 + idx % 16;
     }
     // 8 values of c from c0 + 8 * (lane / 16) on, of index i0 + lane % 16
     static __device__ __forceinline__ typename Frag<E>::type frag(const E* lds, int i0, int c0) {
@@ -250,105 +248,215 @@ struct Tile {
         if constexpr (L == ALONG) {
             return *reinterpret_cast<const typename Frag<E>::type*>(lds + offset(i0 + lane % 16, c0 + lane / 16 * 8));
         } else {
-            constexpr int m = IDX / 16 < 8 ? IDX / 16 - 1 : 7;
             const int c = c0 + lane / 16 * 8 + (lane % 16) / 4;
             // rows c and c + 4 differ in the exclusive-or: two addresses
-            const E* lo = lds + c * IDX + ((i0 / 16) ^ (c & m)) * 16 + lane % 4 * 4;
-            const E* hi = lds + (c + 4) * IDX + ((i0 / 16) ^ ((c + 4) & m)) * 16 + lane % 4 * 4;
-            return read_across<typename Frag<E>::type>(lo, hi);
+            return read_across<typename Frag<E>::type>(lds + offset(i0, c) + lane % 4 * 4,
+                                                       lds + offset(i0, c + 4) + lane % 4 * 4);
         }
     }
     // the tile of `p` whose indices start at i0 (of i_n) and whose c at c0 (of c_n); outside: zero
-    static __device__ __forceinline__ void load(Raw<T> (&raw)[chunks], const T* p, int64_t pitch, int64_t i0,
+    static __device__ __forceinline__ void load(Raw<T> (&raw)[chunks], int tid, const T* p, int64_t pitch, int64_t i0,
                                                 int64_t i_n, int64_t c0, int64_t c_n) {
 #pragma unroll
         for (int n = 0; n < chunks; ++n) {
             int idx, c;
-            place(n, idx, c);
+            place(tid, n, idx, c);
             const int64_t i = i0 + idx, k = c0 + c;
             const int64_t left = L == ALONG ? (i < i_n ? c_n - k : 0) : (k < c_n ? i_n - i : 0);
             const int valid = left >= 8 ? 8 : left > 0 ? (int)left : 0;
             raw[n] = load8<T>(valid ? p + (L == ALONG ? i * pitch + k : k * pitch + i) : p, valid);
         }
     }
-    static __device__ __forceinline__ void store(E* lds, const Raw<T> (&raw)[chunks]) {
+    static __device__ __forceinline__ void store(E* lds, int tid, const Raw<T> (&raw)[chunks]) {
 #pragma unroll
         for (int n = 0; n < chunks; ++n) {
             int idx, c;
-            place(n, idx, c);
+            place(tid, n, idx, c);
             store8<T>(lds + offset(idx, c), plane, raw[n]);
         }
     }
+
+    // Tiles whose c lie inside are read without a branch from addresses found once: indices past the
+    // end read the last ones instead, whose results nobody stores. Not so where such an end cuts a
+    // piece (`whole` is false): those tiles go through load().
+    static __device__ __forceinline__ bool whole(int64_t i0, int64_t i_n) {
+        return L == ALONG || i0 + IDX <= i_n || i_n % 8 == 0;
+    }
+    struct Walk {
+        const T* at[chunks];
+        int64_t step;  // elements from one tile to the next
+
+        __device__ __forceinline__ Walk(int tid, const T* p, int64_t pitch, int64_t i0, int64_t i_n, int64_t c0) {
+#pragma unroll
+            for (int n = 0; n < chunks; ++n) {
+                int idx, c;
+                place(tid, n, idx, c);
+                set(n, p, pitch, i0 + idx, i_n, c0 + c);
+            }
+            step = L == ALONG ? BK : BK * pitch;
+        }
+        __device__ __forceinline__ Walk() {}
+        __device__ __forceinline__ void set(int n, const T* p, int64_t pitch, int64_t i, int64_t i_n, int64_t k) {
+            if constexpr (L == ALONG) at[n] = p + (i < i_n ? i : i_n - 1) * pitch + k;
+            else at[n] = p + k * pitch + (i < i_n ? i : i_n - 8);
+        }
+        __device__ __forceinline__ void next(Raw<T> (&raw)[chunks]) {
+#pragma unroll
+            for (int n = 0; n < chunks; ++n) {
+                __builtin_memcpy(&raw[n], at[n], sizeof(raw[n]));
+                at[n] += step;
+            }
+        }
+    };
+
+    // The same straight into LDS (16-bit types, 16-byte aligned operands): a wave's instruction fills 1 KB in
+    // a row, so the pieces are permuted by the addresses that the lanes read.
+    struct Direct : Walk {
+        __device__ __forceinline__ Direct(const T* p, int64_t pitch, int64_t i0, int64_t i_n, int64_t c0) {
+#pragma unroll
+            for (int n = 0; n < chunks; ++n) {
+                const int slot = n * THREADS + threadIdx.x;  // 16-byte piece of the tile in LDS
+                if constexpr (L == ALONG) {
+                    const int idx = slot / (BK / 8);
+                    this->set(n, p, pitch, i0 + idx, i_n, c0 + ((slot % (BK / 8)) ^ turn(idx)) * 8);
+                } else {
+                    const int c = slot / (IDX / 8), s = slot % (IDX / 8);
+                    this->set(n, p, pitch, i0 + ((s / 2) ^ (c & swap)) * 16 + s % 2 * 8, i_n, c0 + c);
+                }
+            }
+            this->step = L == ALONG ? BK : BK * pitch;
+        }
+        __device__ __forceinline__ void next(E* lds) {
+            typedef __attribute__((address_space(1))) const void gptr;
+            typedef __attribute__((address_space(3))) void lptr;
+            const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+#pragma unroll
+            for (int n = 0; n < chunks; ++n) {
+                __builtin_amdgcn_global_load_lds((gptr*)this->at[n], (lptr*)(lds + (n * THREADS + wave * 64) * 8), 16, 0,
+                                                 0);
+                this->at[n] += this->step;
+            }
+        }
+    };
 };
 
 // ---------------------------------------------------------------------------------------
 // the tile product
 // ---------------------------------------------------------------------------------------
-template <typename T, Layout LR, Layout LB, int BR, int BN>
-struct Product {
+// acc += R * B over the BK of c that a stage holds, for the WR x WN part of the tile at (r0, n0)
+template <typename T, typename TR, typename TB, int NR, int NN>
+__device__ __forceinline__ void multiply(const typename Stage<T>::elem* lr, const typename Stage<T>::elem* lb, int r0,
+                                         int n0, f32x4 (&acc)[NR][NN]) {
     typedef typename Stage<T>::elem E;
-    typedef Tile<T, LR, BR> TR;
-    typedef Tile<T, LB, BN> TB;
-    static constexpr int BK = Stage<T>::bk, P = Stage<T>::planes;
-    static constexpr int waves_r = BR >= 128 ? 2 : 1, waves_n = 4 / waves_r;
-    static constexpr int WR = BR / waves_r, WN = BN / waves_n;
-    static constexpr int NR = WR / 16, NN = WN / 16;
-    static constexpr int lds_elems = P * (TR::plane + TB::plane);
-
-    static __device__ __forceinline__ void step(const E* lr, const E* lb, f32x4 (&acc)[NR][NN]) {
-        const int wave = threadIdx.x / 64;
-        const int r0 = wave / waves_n * WR, n0 = wave % waves_n * WN;
+    constexpr int P = Stage<T>::planes;
 #pragma unroll
-        for (int c = 0; c < BK; c += 32) {
-            typename Frag<E>::type fb[P][NN];
+    for (int c = 0; c < Stage<T>::bk; c += 32) {
+        typename Frag<E>::type fb[P][NN];
 #pragma unroll
-            for (int p = 0; p < P; ++p)
+        for (int p = 0; p < P; ++p)
 #pragma unroll
-                for (int j = 0; j < NN; ++j) fb[p][j] = TB::frag(lb + p * TB::plane, n0 + j * 16, c);
+            for (int j = 0; j < NN; ++j) fb[p][j] = TB::frag(lb + p * TB::plane, n0 + j * 16, c);
 #pragma unroll
-            for (int i = 0; i < NR; ++i) {
-                typename Frag<E>::type fr[P];
+        for (int i = 0; i < NR; ++i) {
+            typename Frag<E>::type fr[P];
 #pragma unroll
-                for (int p = 0; p < P; ++p) fr[p] = TR::frag(lr + p * TR::plane, r0 + i * 16, c);
+            for (int p = 0; p < P; ++p) fr[p] = TR::frag(lr + p * TR::plane, r0 + i * 16, c);
 #pragma unroll
-                for (int j = 0; j < NN; ++j) {
-                    if constexpr (P == 1) {
-                        acc[i][j] = Frag<E>::mfma(fb[0][j], fr[0], acc[i][j]);
-                    } else {  // smallest products first
-                        acc[i][j] = Frag<E>::mfma(fb[2][j], fr[0], acc[i][j]);
-                        acc[i][j] = Frag<E>::mfma(fb[1][j], fr[1], acc[i][j]);
-                        acc[i][j] = Frag<E>::mfma(fb[0][j], fr[2], acc[i][j]);
-                        acc[i][j] = Frag<E>::mfma(fb[1][j], fr[0], acc[i][j]);
-                        acc[i][j] = Frag<E>::mfma(fb[0][j], fr[1], acc[i][j]);
-                        acc[i][j] = Frag<E>::mfma(fb[0][j], fr[0], acc[i][j]);
-                    }
+            for (int j = 0; j < NN; ++j) {
+                if constexpr (P == 1) {
+                    acc[i][j] = Frag<E>::mfma(fb[0][j], fr[0], acc[i][j]);
+                } else {  // smallest products first
+                    acc[i][j] = Frag<E>::mfma(fb[2][j], fr[0], acc[i][j]);
+                    acc[i][j] = Frag<E>::mfma(fb[1][j], fr[1], acc[i][j]);
+                    acc[i][j] = Frag<E>::mfma(fb[0][j], fr[2], acc[i][j]);
+                    acc[i][j] = Frag<E>::mfma(fb[1][j], fr[0], acc[i][j]);
+                    acc[i][j] = Frag<E>::mfma(fb[0][j], fr[1], acc[i][j]);
+                    acc[i][j] = Frag<E>::mfma(fb[0][j], fr[0], acc[i][j]);
                 }
             }
         }
     }
+}
 
-    // acc += R[r0.., c] * B[n0.., c] over c in [c_lo, c_hi). `seen(raw of B's tile)` sees each of them.
+// A workgroup's BR x BN tile, four waves side by side. DIRECT: the operands go straight to LDS, into
+// two stages in turn; else through registers (any alignment, fp32's split) into one.
+template <typename T, Layout LR, Layout LB, int BR, int BN, bool DIRECT>
+struct Product {
+    typedef typename Stage<T>::elem E;
+    typedef Tile<T, LR, BR, kGlThreads> TR;
+    typedef Tile<T, LB, BN, kGlThreads> TB;
+    static constexpr int BK = Stage<T>::bk, P = Stage<T>::planes;
+    static constexpr int waves_r = 2, waves_n = 2;
+    static constexpr int WR = BR / waves_r, WN = BN / waves_n;
+    static constexpr int NR = WR / 16, NN = WN / 16;
+    static constexpr int stage = P * (TR::plane + TB::plane);   // elements
+
+    static __device__ __forceinline__ void step(const E* lds, f32x4 (&acc)[NR][NN]) {
+        const int wave = threadIdx.x / 64;
+        multiply<T, TR, TB, NR, NN>(lds, lds + P * TR::plane, wave / waves_n * WR, wave % waves_n * WN, acc);
+    }
+
+    // acc += R[r0.., c] * B[n0.., c] over c in [c_lo, c_hi). `seen(stage of B)` is called on each stage.
     template <typename F>
-    static __device__ __forceinline__ void run(E* lds, f32x4 (&acc)[NR][NN], const T* r, int64_t r_pitch, int64_t r0,
-                                               int64_t r_n, const T* b, int64_t b_pitch, int64_t n0, int64_t b_n,
-                                               int64_t c_lo, int64_t c_hi, F&& seen) {
-        E* lr = lds;
-        E* lb = lds + P * TR::plane;
-        Raw<T> rr[TR::chunks], rb[TB::chunks];
+    static __device__ __forceinline__ void run(E* s0, E* s1, f32x4 (&acc)[NR][NN], const T* r, int64_t r_pitch,
+                                               int64_t r0, int64_t r_n, const T* b, int64_t b_pitch, int64_t n0,
+                                               int64_t b_n, int64_t c_lo, int64_t c_hi, F&& seen) {
+        const int tid = threadIdx.x;
         if (c_lo >= c_hi) return;
-        TR::load(rr, r, r_pitch, r0, r_n, c_lo, c_hi);
-        TB::load(rb, b, b_pitch, n0, b_n, c_lo, c_hi);
-        for (int64_t c = c_lo; c < c_hi; c += BK) {
-            __syncthreads();  // the last step's reads are done
-            TR::store(lr, rr);
-            TB::store(lb, rb);
-            seen(rb);
-            __syncthreads();
-            if (c + BK < c_hi) {
-                TR::load(rr, r, r_pitch, r0, r_n, c + BK, c_hi);
-                TB::load(rb, b, b_pitch, n0, b_n, c + BK, c_hi);
+        int64_t c = c_lo;
+        Raw<T> rr[TR::chunks], rb[TB::chunks];
+        if (TR::whole(r0, r_n) && TB::whole(n0, b_n)) {
+            const int64_t full = (c_hi - c_lo) / BK;
+            c = c_lo + full * BK;
+            if constexpr (DIRECT) {
+                typename TR::Direct wr(r, r_pitch, r0, r_n, c_lo);
+                typename TB::Direct wb(b, b_pitch, n0, b_n, c_lo);
+                auto fill = [&](E* s) {
+                    wr.next(s);
+                    wb.next(s + TR::plane);
+                };
+                if (full > 0) fill(s0);
+                for (int64_t k = 0; k < full; k += 2) {
+                    __syncthreads();  // stage s0 is filled, and nobody reads s1 any more
+                    if (k + 1 < full) fill(s1);
+                    seen(s0 + TR::plane);
+                    step(s0, acc);
+                    if (k + 1 >= full) break;
+                    __syncthreads();
+                    if (k + 2 < full) fill(s0);
+                    seen(s1 + TR::plane);
+                    step(s1, acc);
+                }
+            } else {
+                typename TR::Walk wr(tid, r, r_pitch, r0, r_n, c_lo);
+                typename TB::Walk wb(tid, b, b_pitch, n0, b_n, c_lo);
+                if (full > 0) {
+                    wr.next(rr);
+                    wb.next(rb);
+                }
+                for (int64_t k = 0; k < full; ++k) {
+                    __syncthreads();  // the last step's reads are done
+                    TR::store(s0, tid, rr);
+                    TB::store(s0 + P * TR::plane, tid, rb);
+                    __syncthreads();
+                    if (k + 1 < full) {
+                        wr.next(rr);
+                        wb.next(rb);
+                    }
+                    seen(s0 + P * TR::plane);
+                    step(s0, acc);
+                }
             }
-            step(lr, lb, acc);
+        }
+        for (; c < c_hi; c += BK) {  // what is left of c, and tiles at an end that cuts a piece
+            TR::load(rr, tid, r, r_pitch, r0, r_n, c, c_hi);
+            TB::load(rb, tid, b, b_pitch, n0, b_n, c, c_hi);
+            __syncthreads();
+            TR::store(s0, tid, rr);
+            TB::store(s0 + P * TR::plane, tid, rb);
+            __syncthreads();
+            seen(s0 + P * TR::plane);
+            step(s0, acc);
         }
     }
 
@@ -380,73 +488,170 @@ __device__ __forceinline__ void store4(T* p, const f32x4& v, int valid) {
     }
 }
 
+// Four results of the forward or input gradient: what is not finite in fp32 again from the operands,
+// the bias, and the rounding to T.
+template <typename T, Layout LB>
+__device__ __forceinline__ void finish4(const GroupedArgs& a, const Item& it, const T* b, int64_t row, int64_t col,
+                                        f32x4& v) {
+    if (row >= it.hi || col >= a.cols) return;
+    const int valid = a.cols - col < 4 ? (int)(a.cols - col) : 4;
+    const bool owned = it.group < a.groups;
+    if constexpr (sizeof(T) == 4) {
+        const T* r = (const T*)a.r;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (finite(v[k]) || k >= valid || !owned) continue;
+            float s = 0.0f;
+            for (int c = 0; c < a.cc; ++c)
+                s = __builtin_fmaf(r[row * a.r_pitch + c], LB == ALONG ? b[(col + k) * a.b_pitch + c]
+                                                                       : b[c * a.b_pitch + col + k], s);
+            v[k] = s;
+        }
+    }
+    if (owned && a.bias) {
+        const T* bias = (const T*)a.bias + (int64_t)it.group * a.cols;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (k < valid) v[k] += (float)bias[col + k];
+    }
+    store4<T>((T*)a.out + row * a.cols + col, v, valid);
+}
+
 // forward (LB = ACROSS) and input gradient (LB = ALONG): a workgroup per row tile and column tile
-template <typename T, Layout LB, int BR, int BN>
-__global__ __launch_bounds__(kGlThreads) void grouped_rows_kernel(GroupedArgs a) {
-    typedef Product<T, ALONG, LB, BR, BN> X;
-    __shared__ __attribute__((aligned(16))) typename X::E lds[X::lds_elems];
-    const Item it = find_item(a, blockIdx.x / a.col_tiles, BR, 0, true);
+template <typename T, Layout LB, int BR, int BN, bool DIRECT>
+__global__ __launch_bounds__(kGlThreads, 2) void grouped_rows_kernel(GroupedArgs a) {
+    typedef Product<T, ALONG, LB, BR, BN, DIRECT> X;
+    __shared__ __attribute__((aligned(16))) typename X::E s0[X::stage];
+    __shared__ __attribute__((aligned(16))) typename X::E s1[DIRECT ? X::stage : 8];
+    const Item it = find_item<kGlThreads>(a, blockIdx.x / a.col_tiles, BR, 0, true);
     if (it.group < 0) return;
     const int64_t n0 = (int64_t)(blockIdx.x % a.col_tiles) * BN;
     const int64_t r0 = it.lo + (int64_t)it.part * BR;
     f32x4 acc[X::NR][X::NN] = {};
-    const bool owned = it.group < a.groups;
+    const T* b = (const T*)a.b + (int64_t)it.group * a.b_group;
+    if (it.group < a.groups)
+        X::run(s0, s1, acc, (const T*)a.r, a.r_pitch, r0, it.hi, b, a.b_pitch, n0, a.cols, 0, a.cc, [](auto*) {});
+    X::each(acc, [&](int ir, int in, f32x4& v) { finish4<T, LB>(a, it, b, r0 + ir, n0 + in, v); });
+}
+
+// The same for few rows a group, where the time goes into reading the weights: tiles of 32 rows and 64
+// columns, and the WAVES waves of a workgroup split c, each with a stage of its own and two more in
+// its registers on their way from memory, so that no wave waits for another before the end.
+template <typename T, Layout LB, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, 2) void grouped_few_rows_kernel(GroupedArgs a) {
+    constexpr int BR = 32, BN = 64, NR = BR / 16, NN = BN / 16, P = Stage<T>::planes, BK = Stage<T>::bk;
+    typedef typename Stage<T>::elem E;
+    typedef Tile<T, ALONG, BR, 64> TR;
+    typedef Tile<T, LB, BN, 64> TB;
+    constexpr int stage = P * (TR::plane + TB::plane);
+    __shared__ __attribute__((aligned(16))) E lds[WAVES * stage];
+    static_assert(sizeof(E) * stage >= BR * BN * sizeof(float), "a wave's results fit its stage");
+    const Item it = find_item<WAVES * 64>(a, blockIdx.x / a.col_tiles, BR, 0, true);
+    if (it.group < 0) return;
+    const int64_t n0 = (int64_t)(blockIdx.x % a.col_tiles) * BN;
+    const int64_t r0 = it.lo + (int64_t)it.part * BR;
+    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
     const T* r = (const T*)a.r;
-    const T* b = (const T*)a.b + (owned ? (int64_t)it.group * a.b_group : 0);
-    if (owned)
-        X::run(lds, acc, r, a.r_pitch, r0, it.hi, b, a.b_pitch, n0, a.cols, 0, a.cc, [](auto&) {});
-    const T* bias = owned && a.bias ? (const T*)a.bias + (int64_t)it.group * a.cols : nullptr;
-    X::each(acc, [&](int ir, int in, f32x4& v) {
-        const int64_t row = r0 + ir, col = n0 + in;
-        if (row >= it.hi || col >= a.cols) return;
-        const int valid = a.cols - col < 4 ? (int)(a.cols - col) : 4;
-        if constexpr (sizeof(T) == 4) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                if (finite(v[k]) || k >= valid || !owned) continue;
-                float s = 0.0f;
-                for (int c = 0; c < a.cc; ++c)
-                    s = __builtin_fmaf(r[row * a.r_pitch + c],
-                                       LB == ALONG ? b[(col + k) * a.b_pitch + c] : b[c * a.b_pitch + col + k], s);
-                v[k] = s;
+    const T* b = (const T*)a.b + (int64_t)it.group * a.b_group;
+    E* s = lds + wave * stage;
+    f32x4 acc[NR][NN] = {};
+    if (it.group < a.groups) {
+        const int steps = (a.cc + BK - 1) / BK, share = (steps + WAVES - 1) / WAVES;
+        const int64_t c_lo = (int64_t)wave * share * BK;
+        const int64_t c_hi = c_lo + (int64_t)share * BK < a.cc ? c_lo + (int64_t)share * BK : a.cc;
+        Raw<T> rr[2][TR::chunks], rb[2][TB::chunks];
+        auto put = [&](int q) {  // the wave's LDS instructions run in order: no barrier
+            TR::store(s, lane, rr[q]);
+            TB::store(s + P * TR::plane, lane, rb[q]);
+            __builtin_amdgcn_wave_barrier();
+        };
+        auto use = [&] {
+            multiply<T, TR, TB, NR, NN>(s, s + P * TR::plane, 0, 0, acc);
+            __builtin_amdgcn_wave_barrier();
+        };
+        int64_t c = c_lo;
+        if (TB::whole(n0, a.cols) && c_lo < c_hi) {
+            const int64_t full = (c_hi - c_lo) / BK;
+            c = c_lo + full * BK;
+            typename TR::Walk wr(lane, r, a.r_pitch, r0, it.hi, c_lo);
+            typename TB::Walk wb(lane, b, a.b_pitch, n0, a.cols, c_lo);
+            auto get = [&](int q) {
+                wr.next(rr[q]);
+                wb.next(rb[q]);
+            };
+            if (full > 0) get(0);
+            if (full > 1) get(1);
+            for (int64_t k = 0; k < full; k += 2) {
+                put(0);
+                if (k + 2 < full) get(0);
+                use();
+                if (k + 1 >= full) break;
+                put(1);
+                if (k + 3 < full) get(1);
+                use();
             }
         }
-        if (bias) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (k < valid) v[k] += (float)bias[col + k];
+        for (; c < c_hi; c += BK) {
+            TR::load(rr[0], lane, r, a.r_pitch, r0, it.hi, c, c_hi);
+            TB::load(rb[0], lane, b, a.b_pitch, n0, a.cols, c, c_hi);
+            put(0);
+            use();
         }
-        store4<T>((T*)a.out + row * a.cols + col, v, valid);
-    });
+    }
+    // the waves' parts, added in order
+    float* mine = reinterpret_cast<float*>(s);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NR; ++i)
+#pragma unroll
+        for (int j = 0; j < NN; ++j)
+            *reinterpret_cast<f32x4*>(mine + (i * 16 + lane % 16) * BN + j * 16 + lane / 16 * 4) = acc[i][j];
+    __syncthreads();
+    for (int q = threadIdx.x; q < BR * BN / 4; q += WAVES * 64) {
+        const int ir = q / (BN / 4), in = q % (BN / 4) * 4;
+        f32x4 v = {};
+        for (int w = 0; w < WAVES; ++w)
+            v += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + w * stage) + ir * BN + in);
+        finish4<T, LB>(a, it, b, r0 + ir, n0 + in, v);
+    }
 }
 
 // weight gradient: a workgroup per chunk of a group's rows and tile of the weight. A group of one
 // chunk is written as it is; the chunks of a longer one leave fp32 slabs for the kernel below.
-template <typename T, int BR, int BN>
-__global__ __launch_bounds__(kGlThreads) void grouped_wgrad_kernel(GroupedArgs a) {
-    typedef Product<T, ACROSS, ACROSS, BR, BN> X;
-    __shared__ __attribute__((aligned(16))) typename X::E lds[X::lds_elems];
+template <typename T, int BR, int BN, bool DIRECT>
+__global__ __launch_bounds__(kGlThreads, 2) void grouped_wgrad_kernel(GroupedArgs a) {
+    typedef Product<T, ACROSS, ACROSS, BR, BN, DIRECT> X;
+    __shared__ __attribute__((aligned(16))) typename X::E s0[X::stage];
+    __shared__ __attribute__((aligned(16))) typename X::E s1[DIRECT ? X::stage : 8];
     const int tiles = a.row_tiles * a.col_tiles;
     const int64_t id = blockIdx.x / tiles;
     const int tile = blockIdx.x % tiles;
-    const Item it = find_item(a, id, a.chunk, 1, false);
+    const Item it = find_item<kGlThreads>(a, id, a.chunk, 1, false);
     if (it.group < 0) return;
     const int64_t r0 = (int64_t)(tile / a.col_tiles) * BR, n0 = (int64_t)(tile % a.col_tiles) * BN;
     const int64_t c_lo = it.lo + (int64_t)it.part * a.chunk;
     const int64_t c_hi = c_lo + a.chunk < it.hi ? c_lo + a.chunk : it.hi;
     f32x4 acc[X::NR][X::NN] = {};
-    float col_sum[8] = {};  // of the columns that this thread stages: the same in every piece
+    float col_sum[8] = {};  // of the columns of this thread's pieces: the same in every piece
     const bool want_b = a.dbias && r0 == 0;
     const T* r = (const T*)a.r;
     const T* b = (const T*)a.b;
-    X::run(lds, acc, r, a.r_pitch, r0, a.out_rows, b, a.b_pitch, n0, a.cols, c_lo, c_hi, [&](auto& raw) {
+    X::run(s0, s1, acc, r, a.r_pitch, r0, a.out_rows, b, a.b_pitch, n0, a.cols, c_lo, c_hi, [&](auto* stage) {
         if (!want_b) return;
 #pragma unroll
         for (int n = 0; n < X::TB::chunks; ++n) {
-            T e[8];
-            __builtin_memcpy(e, &raw[n], sizeof(e));
+            int idx, c;
+            X::TB::place(threadIdx.x, n, idx, c);
+            typename VecOf<typename X::E, 8>::type e[X::P];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) col_sum[k] += (float)e[k];
+            for (int p = 0; p < X::P; ++p)
+                e[p] = *reinterpret_cast<const typename VecOf<typename X::E, 8>::type*>(stage + p * X::TB::plane +
+                                                                                       X::TB::offset(idx, c));
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                if constexpr (X::P == 1) col_sum[k] += (float)e[0][k];
+                else col_sum[k] += ((float)e[X::P - 1][k] + (float)e[1][k]) + (float)e[0][k];  // the value, exactly
+            }
         }
     });
     const int64_t size = (int64_t)a.out_rows * a.cols;
@@ -470,11 +675,10 @@ __global__ __launch_bounds__(kGlThreads) void grouped_wgrad_kernel(GroupedArgs a
         else store4<T>((T*)a.out + (int64_t)it.group * size + row * a.cols + col, v, valid);
     });
     if (!want_b) return;
-    // the threads that staged the same columns, in order
+    // the threads whose pieces have the same columns, in order
     constexpr int teams = kGlThreads / (BN / 8);
-    static_assert(X::TB::chunks * kGlThreads * 8 == BN * X::BK, "a thread's pieces share their columns");
-    float* sums = reinterpret_cast<float*>(lds);
-    static_assert(sizeof(lds) >= teams * BN * sizeof(float), "the column sums fit the stage");
+    float* sums = reinterpret_cast<float*>(s0);
+    static_assert(sizeof(s0) >= teams * BN * sizeof(float), "the column sums fit the stage");
     __syncthreads();
     const int team = threadIdx.x / (BN / 8), c8 = threadIdx.x % (BN / 8) * 8;
 #pragma unroll
@@ -483,6 +687,12 @@ __global__ __launch_bounds__(kGlThreads) void grouped_wgrad_kernel(GroupedArgs a
     for (int c = threadIdx.x; c < BN && n0 + c < a.cols; c += kGlThreads) {
         float s = sums[c];
         for (int q = 1; q < teams; ++q) s += sums[q * BN + c];
+        if constexpr (sizeof(T) == 4) {  // an infinity's pieces are not numbers
+            if (!finite(s)) {
+                s = 0.0f;
+                for (int64_t i = c_lo; i < c_hi; ++i) s += b[i * a.b_pitch + n0 + c];
+            }
+        }
         if (part) part[size + n0 + c] = s;
         else ((T*)a.dbias)[(int64_t)it.group * a.cols + n0 + c] = (T)s;
     }
@@ -526,6 +736,7 @@ __global__ __launch_bounds__(kGlThreads) void grouped_slabs_kernel(GroupedArgs a
 // host
 // ---------------------------------------------------------------------------------------
 constexpr int kTile = 128;
+constexpr int kFewRows = 32;  // rows a group on average, up to which grouped_few_rows_kernel runs
 
 // Rows of a chunk of the weight gradient: whole groups where the weight alone has tiles enough to
 // fill the chip, else as many rows as leave about four workgroups per CU.
@@ -549,24 +760,57 @@ int32_t check_grouped(int64_t rows, int64_t groups, int64_t k, int64_t n, int32_
     return MPGNN_OK;
 }
 
+// operands that go straight to LDS: 16-bit, their rows and groups at multiples of 16 bytes
 template <typename T>
-int32_t rows_product(GroupedArgs a, bool dgrad, hipStream_t strm) {
-    a.col_tiles = (a.cols + kTile - 1) / kTile;
-    const int64_t blocks = (a.rows / kTile + a.groups + 2) * a.col_tiles;
+bool direct_ok(const GroupedArgs& a) {
+    return sizeof(T) == 2 && aligned16(a.r) && aligned16(a.b) && a.r_pitch % 8 == 0 && a.b_pitch % 8 == 0 &&
+           a.b_group % 8 == 0;
+}
+
+template <typename T, Layout LB, int WAVES>
+void launch_few(GroupedArgs a, unsigned blocks, hipStream_t strm) {
+    hipLaunchKernelGGL((grouped_few_rows_kernel<T, LB, WAVES>), dim3(blocks), dim3(WAVES * 64), 0, strm, a);
+}
+
+template <typename T, Layout LB, bool DIRECT>
+void launch_rows(GroupedArgs a, unsigned blocks, hipStream_t strm) {
+    hipLaunchKernelGGL((grouped_rows_kernel<T, LB, kTile, kTile, DIRECT>), dim3(blocks), dim3(kGlThreads), 0, strm, a);
+}
+
+template <typename T, Layout LB>
+int32_t rows_product(GroupedArgs a, hipStream_t strm) {
+    const bool few = a.rows <= (int64_t)kFewRows * a.groups;
+    const int br = few ? 32 : kTile, bn = few ? 64 : kTile;
+    a.col_tiles = (a.cols + bn - 1) / bn;
+    const int64_t blocks = (a.rows / br + a.groups + 2) * a.col_tiles;
     if (blocks > INT32_MAX) return unsupported("grouped linear: more than 2^31 tiles");
-    if (dgrad)
-        hipLaunchKernelGGL((grouped_rows_kernel<T, ALONG, kTile, kTile>), dim3((unsigned)blocks), dim3(kGlThreads), 0,
-                           strm, a);
-    else
-        hipLaunchKernelGGL((grouped_rows_kernel<T, ACROSS, kTile, kTile>), dim3((unsigned)blocks), dim3(kGlThreads), 0,
-                           strm, a);
+    if (few) {
+        // workgroups that find rows: at most one per row and column tile; below two per CU a workgroup
+        // takes eight waves to have as many bytes on their way
+        const int64_t busy = std::min<int64_t>(a.rows, a.rows / br + a.groups) * a.col_tiles;
+        if (busy < 512) launch_few<T, LB, 8>(a, (unsigned)blocks, strm);
+        else launch_few<T, LB, 4>(a, (unsigned)blocks, strm);
+    } else {
+        if constexpr (sizeof(T) == 2) {
+            if (direct_ok<T>(a)) {
+                launch_rows<T, LB, true>(a, (unsigned)blocks, strm);
+                return launch_status("grouped linear: the launch failed");
+            }
+        }
+        launch_rows<T, LB, false>(a, (unsigned)blocks, strm);
+    }
     return launch_status("grouped linear: the launch failed");
+}
+
+template <typename T>
+int32_t rows_either(const GroupedArgs& a, bool dgrad, hipStream_t strm) {
+    return dgrad ? rows_product<T, ALONG>(a, strm) : rows_product<T, ACROSS>(a, strm);
 }
 
 int32_t rows_by_type(const GroupedArgs& a, int32_t dtype, bool dgrad, hipStream_t strm) {
     if (a.rows == 0) return MPGNN_OK;
-    if (dtype == MPGNN_F32) return rows_product<float>(a, dgrad, strm);
-    return dtype == MPGNN_BF16 ? rows_product<__bf16>(a, dgrad, strm) : rows_product<_Float16>(a, dgrad, strm);
+    if (dtype == MPGNN_F32) return rows_either<float>(a, dgrad, strm);
+    return dtype == MPGNN_BF16 ? rows_either<__bf16>(a, dgrad, strm) : rows_either<_Float16>(a, dgrad, strm);
 }
 
 template <typename T>
@@ -576,7 +820,16 @@ int32_t wgrad_product(GroupedArgs a, hipStream_t strm) {
     a.items = wgrad_items(a.rows, a.groups, a.chunk);
     const int64_t blocks = a.items * a.row_tiles * a.col_tiles;
     if (blocks > INT32_MAX) return unsupported("grouped linear: more than 2^31 tiles");
-    hipLaunchKernelGGL((grouped_wgrad_kernel<T, kTile, kTile>), dim3((unsigned)blocks), dim3(kGlThreads), 0, strm, a);
+    bool direct = false;
+    if constexpr (sizeof(T) == 2) {
+        direct = direct_ok<T>(a);
+        if (direct)
+            hipLaunchKernelGGL((grouped_wgrad_kernel<T, kTile, kTile, true>), dim3((unsigned)blocks), dim3(kGlThreads),
+                               0, strm, a);
+    }
+    if (!direct)
+        hipLaunchKernelGGL((grouped_wgrad_kernel<T, kTile, kTile, false>), dim3((unsigned)blocks), dim3(kGlThreads), 0,
+                           strm, a);
     if (a.rows > a.chunk) {
         const int64_t slab = (int64_t)a.out_rows * a.cols + a.cols;
         const int pieces = (int)std::min<int64_t>(64, (slab + kGlThreads * 4 - 1) / (kGlThreads * 4));
