@@ -106,6 +106,11 @@ __device__ __forceinline__ int64_t ptr_at(const GroupedArgs& a, int g) {
     return v < 0 ? 0 : v > a.rows ? a.rows : v;  // no ptr, however wrong, leads outside the tensors
 }
 
+__device__ __forceinline__ int64_t scalar(int64_t v) {
+    return (int64_t)((uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 |
+                     (unsigned)__builtin_amdgcn_readfirstlane((int)v));
+}
+
 struct Item {
     int group;    // -1: none; groups: rows that belong to no group
     int part;     // which tile (chunk) of the group
@@ -159,7 +164,13 @@ __device__ __forceinline__ Item find_item(const GroupedArgs& a, int64_t id, int 
         if (base > id) break;
     }
     __syncthreads();
-    return s_item;
+    Item it = s_item;  // the same in every lane: into scalar registers
+    it.group = __builtin_amdgcn_readfirstlane(it.group);
+    it.part = __builtin_amdgcn_readfirstlane(it.part);
+    it.parts = __builtin_amdgcn_readfirstlane(it.parts);
+    it.lo = scalar(it.lo);
+    it.hi = scalar(it.hi);
+    return it;
 }
 
 // ---------------------------------------------------------------------------------------
@@ -217,10 +228,9 @@ __device__ __forceinline__ void store8(typename Stage<T>::elem* dst, int plane_s
 }
 
 // A tile of IDX indices x BK of c, staged by THREADS threads.
-template <typename T, Layout L, int IDX, int THREADS>
+template <typename T, Layout L, int IDX, int BK, int THREADS>
 struct Tile {
     typedef typename Stage<T>::elem E;
-    static constexpr int BK = Stage<T>::bk;
     static constexpr int plane = IDX * BK;                      // elements
     static constexpr int chunks = IDX * BK / 8 / THREADS;       // 8-element pieces per thread
     static_assert(chunks >= 1 && chunks * THREADS * 8 == plane, "the threads' pieces make up the tile");
@@ -236,22 +246,27 @@ struct Tile {
             idx = id % (IDX / 8) * 8;
         }
     }
-    static constexpr int swap = IDX / 16 < 8 ? IDX / 16 - 1 : 7;  // ACROSS: bits of c that move a 32-byte block
+    static_assert(L == ALONG || IDX % 64 == 0, "ACROSS: the four 32-byte blocks of 128 bytes trade places");
     static __device__ __forceinline__ int turn(int idx) { return BK == 64 ? idx & 7 : (idx >> 1) & 3; }  // ALONG
     static __device__ __forceinline__ int offset(int idx, int c) {
         if constexpr (L == ALONG) return idx * BK + ((c / 8) ^ turn(idx)) * 8 + c % 8;
-        else return c * IDX + ((idx / 16) ^ (c & swap)) * 16 + idx % 16;
+        else return c * IDX + ((idx / 16) ^ (c & 3)) * 16 + idx % 16;
     }
-    // 8 values of c from c0 + 8 * (lane / 16) on, of index i0 + lane % 16
-    static __device__ __forceinline__ typename Frag<E>::type frag(const E* lds, int i0, int c0) {
+    // The fragment of indices i0 + i .. + 15 and c .. c + 31, of which a lane has 8 values of c from c + 8 *
+    // (lane / 16) on, of index i0 + i + lane % 16: at(i0) is the lane's place for i = c = 0, and i and c,
+    // constants in the unrolled loops, change bits of it that it leaves alone (i0: a multiple of
+    // 64, or of 32 with i < 32).
+    static __device__ __forceinline__ unsigned at(int i0) {
         const int lane = threadIdx.x % 64;
+        return L == ALONG ? offset(i0 + lane % 16, lane / 16 * 8)
+                          : offset(i0, lane / 16 * 8 + (lane % 16) / 4) + lane % 4 * 4;
+    }
+    static __device__ __forceinline__ typename Frag<E>::type frag(const E* lds, unsigned at, int i, int c) {
         if constexpr (L == ALONG) {
-            return *reinterpret_cast<const typename Frag<E>::type*>(lds + offset(i0 + lane % 16, c0 + lane / 16 * 8));
+            return *reinterpret_cast<const typename Frag<E>::type*>(lds + (at ^ c) + i * BK);
         } else {
-            const int c = c0 + lane / 16 * 8 + (lane % 16) / 4;
-            // rows c and c + 4 differ in the exclusive-or: two addresses
-            return read_across<typename Frag<E>::type>(lds + offset(i0, c) + lane % 4 * 4,
-                                                       lds + offset(i0, c + 4) + lane % 4 * 4);
+            const E* p = lds + (at ^ (i & 48)) + i / 64 * 64 + c * IDX;
+            return read_across<typename Frag<E>::type>(p, p + 4 * IDX);
         }
     }
     // the tile of `p` whose indices start at i0 (of i_n) and whose c at c0 (of c_n); outside: zero
@@ -273,6 +288,21 @@ struct Tile {
             int idx, c;
             place(tid, n, idx, c);
             store8<T>(lds + offset(idx, c), plane, raw[n]);
+        }
+    }
+
+    // load() and store() a piece at a time: the few registers of what runs once a tile
+    static __device__ __forceinline__ void copy(E* lds, int tid, const T* p, int64_t pitch, int64_t i0, int64_t i_n,
+                                                int64_t c0, int64_t c_n) {
+#pragma unroll 1
+        for (int n = 0; n < chunks; ++n) {
+            int idx, c;
+            place(tid, n, idx, c);
+            const int64_t i = i0 + idx, k = c0 + c;
+            const int64_t left = L == ALONG ? (i < i_n ? c_n - k : 0) : (k < c_n ? i_n - i : 0);
+            const int valid = left >= 8 ? 8 : left > 0 ? (int)left : 0;
+            store8<T>(lds + offset(idx, c), plane,
+                      load8<T>(valid ? p + (L == ALONG ? i * pitch + k : k * pitch + i) : p, valid));
         }
     }
 
@@ -310,32 +340,42 @@ struct Tile {
     };
 
     // The same straight into LDS (16-bit types, 16-byte aligned operands): a wave's instruction fills 1 KB in
-    // a row, so the pieces are permuted by the addresses that the lanes read.
-    struct Direct : Walk {
+    // a row, so the pieces are permuted by the addresses that the lanes read, bytes from a uniform base.
+    struct Direct {
+        unsigned at[chunks];
+        unsigned wave_at;  // the wave's part of an instruction's pieces in LDS, bytes
+        const T* base;
+        int64_t step;
+
         __device__ __forceinline__ Direct(const T* p, int64_t pitch, int64_t i0, int64_t i_n, int64_t c0) {
+            wave_at = __builtin_amdgcn_readfirstlane(threadIdx.x / 64) * 1024;
+            const int end = i_n - i0 < IDX ? (int)(i_n - i0) : IDX;  // at least 1; ACROSS: at least 8
 #pragma unroll
             for (int n = 0; n < chunks; ++n) {
                 const int slot = n * THREADS + threadIdx.x;  // 16-byte piece of the tile in LDS
                 if constexpr (L == ALONG) {
                     const int idx = slot / (BK / 8);
-                    this->set(n, p, pitch, i0 + idx, i_n, c0 + ((slot % (BK / 8)) ^ turn(idx)) * 8);
+                    at[n] = (unsigned)((idx < end ? idx : end - 1) * (int)pitch + ((slot % (BK / 8)) ^ turn(idx)) * 8) * 2;
                 } else {
                     const int c = slot / (IDX / 8), s = slot % (IDX / 8);
-                    this->set(n, p, pitch, i0 + ((s / 2) ^ (c & swap)) * 16 + s % 2 * 8, i_n, c0 + c);
+                    const int idx = ((s / 2) ^ (c & 3)) * 16 + s % 2 * 8;
+                    at[n] = (unsigned)(c * (int)pitch + (idx < end ? idx : end - 8)) * 2;
                 }
             }
-            this->step = L == ALONG ? BK : BK * pitch;
+            base = L == ALONG ? p + i0 * pitch + c0 : p + c0 * pitch + i0;
+            step = L == ALONG ? BK : BK * pitch;
         }
+        // (written out, as the compiler would wait for every load before it reads any stage)
         __device__ __forceinline__ void next(E* lds) {
-            typedef __attribute__((address_space(1))) const void gptr;
-            typedef __attribute__((address_space(3))) void lptr;
-            const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+            typedef __attribute__((address_space(3))) E* lptr;
+            const unsigned to = (unsigned)(unsigned long long)(lptr)lds + wave_at;
 #pragma unroll
-            for (int n = 0; n < chunks; ++n) {
-                __builtin_amdgcn_global_load_lds((gptr*)this->at[n], (lptr*)(lds + (n * THREADS + wave * 64) * 8), 16, 0,
-                                                 0);
-                this->at[n] += this->step;
-            }
+            for (int n = 0; n < chunks; ++n)
+                asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1"
+                             :
+                             : "v"(at[n]), "s"(base), "s"(to + n * THREADS * 16)
+                             : "memory");
+            base += step;
         }
     };
 };
@@ -344,23 +384,26 @@ struct Tile {
 // the tile product
 // ---------------------------------------------------------------------------------------
 // acc += R * B over the BK of c that a stage holds, for the WR x WN part of the tile at (r0, n0)
-template <typename T, typename TR, typename TB, int NR, int NN>
+template <typename T, typename TR, typename TB, int BK, int NR, int NN>
 __device__ __forceinline__ void multiply(const typename Stage<T>::elem* lr, const typename Stage<T>::elem* lb, int r0,
                                          int n0, f32x4 (&acc)[NR][NN]) {
     typedef typename Stage<T>::elem E;
     constexpr int P = Stage<T>::planes;
+    // kept from being found once for every fragment and stage: more registers than there are
+    unsigned at_r = TR::at(r0), at_b = TB::at(n0);
+    asm volatile("" : "+v"(at_r), "+v"(at_b));
 #pragma unroll
-    for (int c = 0; c < Stage<T>::bk; c += 32) {
+    for (int c = 0; c < BK; c += 32) {
         typename Frag<E>::type fb[P][NN];
 #pragma unroll
         for (int p = 0; p < P; ++p)
 #pragma unroll
-            for (int j = 0; j < NN; ++j) fb[p][j] = TB::frag(lb + p * TB::plane, n0 + j * 16, c);
+            for (int j = 0; j < NN; ++j) fb[p][j] = TB::frag(lb + p * TB::plane, at_b, j * 16, c);
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
             typename Frag<E>::type fr[P];
 #pragma unroll
-            for (int p = 0; p < P; ++p) fr[p] = TR::frag(lr + p * TR::plane, r0 + i * 16, c);
+            for (int p = 0; p < P; ++p) fr[p] = TR::frag(lr + p * TR::plane, at_r, i * 16, c);
 #pragma unroll
             for (int j = 0; j < NN; ++j) {
                 if constexpr (P == 1) {
@@ -378,63 +421,78 @@ __device__ __forceinline__ void multiply(const typename Stage<T>::elem* lr, cons
     }
 }
 
-// A workgroup's BR x BN tile, four waves side by side. DIRECT: the operands go straight to LDS, into
-// two stages in turn; else through registers (any alignment, fp32's split) into one.
-template <typename T, Layout LR, Layout LB, int BR, int BN, bool DIRECT>
+// Every load that a wave has sent to LDS is there, and every wave of the workgroup is here.
+__device__ __forceinline__ void arrive() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// A workgroup's BR x BN tile, its waves side by side. DIRECT: the operands go straight to LDS, into
+// two stages in turn, of which one is on its way while the other is multiplied. Else through
+// registers (any alignment, fp32's split) into one.
+template <typename T, Layout LR, Layout LB, int BR, int BN, int THREADS, bool DIRECT>
 struct Product {
     typedef typename Stage<T>::elem E;
-    typedef Tile<T, LR, BR, kGlThreads> TR;
-    typedef Tile<T, LB, BN, kGlThreads> TB;
     static constexpr int BK = Stage<T>::bk, P = Stage<T>::planes;
-    static constexpr int waves_r = 2, waves_n = 2;
+    typedef Tile<T, LR, BR, BK, THREADS> TR;
+    typedef Tile<T, LB, BN, BK, THREADS> TB;
+    static constexpr int waves_r = 2, waves_n = THREADS / 64 / waves_r;
     static constexpr int WR = BR / waves_r, WN = BN / waves_n;
     static constexpr int NR = WR / 16, NN = WN / 16;
     static constexpr int stage = P * (TR::plane + TB::plane);   // elements
 
     static __device__ __forceinline__ void step(const E* lds, f32x4 (&acc)[NR][NN]) {
         const int wave = threadIdx.x / 64;
-        multiply<T, TR, TB, NR, NN>(lds, lds + P * TR::plane, wave / waves_n * WR, wave % waves_n * WN, acc);
+        multiply<T, TR, TB, BK, NR, NN>(lds, lds + P * TR::plane, wave / waves_n * WR, wave % waves_n * WN, acc);
     }
 
     // acc += R[r0.., c] * B[n0.., c] over c in [c_lo, c_hi). `seen(stage of B)` is called on each stage.
     template <typename F>
     static __device__ __forceinline__ void run(E* s0, E* s1, f32x4 (&acc)[NR][NN], const T* r, int64_t r_pitch,
-                                               int64_t r0, int64_t r_n, const T* b, int64_t b_pitch, int64_t n0,
-                                               int64_t b_n, int64_t c_lo, int64_t c_hi, F&& seen) {
+                                               int64_t r0, int64_t r_n, const T* b, int64_t b_pitch,
+                                               int64_t n0, int64_t b_n, int64_t c_lo, int64_t c_hi, F&& seen) {
         const int tid = threadIdx.x;
         if (c_lo >= c_hi) return;
         int64_t c = c_lo;
-        Raw<T> rr[TR::chunks], rb[TB::chunks];
-        if (TR::whole(r0, r_n) && TB::whole(n0, b_n)) {
-            const int64_t full = (c_hi - c_lo) / BK;
-            c = c_lo + full * BK;
-            if constexpr (DIRECT) {
+        const bool whole = TR::whole(r0, r_n) && TB::whole(n0, b_n);
+        const int full = __builtin_amdgcn_readfirstlane(whole ? (int)((c_hi - c_lo) / BK) : 0);
+        c = c_lo + (int64_t)full * BK;
+        if constexpr (DIRECT) {
+            if (full > 0) {
                 typename TR::Direct wr(r, r_pitch, r0, r_n, c_lo);
                 typename TB::Direct wb(b, b_pitch, n0, b_n, c_lo);
                 auto fill = [&](E* s) {
                     wr.next(s);
                     wb.next(s + TR::plane);
                 };
-                if (full > 0) fill(s0);
-                for (int64_t k = 0; k < full; k += 2) {
-                    __syncthreads();  // stage s0 is filled, and nobody reads s1 any more
-                    if (k + 1 < full) fill(s1);
-                    seen(s0 + TR::plane);
-                    step(s0, acc);
-                    if (k + 1 >= full) break;
-                    __syncthreads();
-                    if (k + 2 < full) fill(s0);
-                    seen(s1 + TR::plane);
-                    step(s1, acc);
+                fill(s0);
+                auto turn = [&](int k, E* now, E* next) {
+                    arrive();  // stage `now` is filled, and nobody reads `next` any more
+                    if (k + 1 < full) fill(next);
+                    seen(now + TR::plane);
+                    step(now, acc);
+                };
+                int k = 0;
+                for (; k + 2 <= full; k += 2) {
+                    turn(k, s0, s1);
+                    turn(k + 1, s1, s0);
                 }
-            } else {
+                // (no exit from the middle of the loop: the accumulators would have a copy per exit)
+                if (k < full) turn(k, s0, s1);
+            }
+            for (; c < c_hi; c += BK) {  // what is left of c, and tiles at an end that cuts a piece
+                __syncthreads();
+                TR::copy(s0, tid, r, r_pitch, r0, r_n, c, c_hi);
+                TB::copy(s0 + TR::plane, tid, b, b_pitch, n0, b_n, c, c_hi);
+                __syncthreads();
+                seen(s0 + TR::plane);
+                step(s0, acc);
+            }
+        } else {
+            Raw<T> rr[TR::chunks], rb[TB::chunks];
+            if (full > 0) {
                 typename TR::Walk wr(tid, r, r_pitch, r0, r_n, c_lo);
                 typename TB::Walk wb(tid, b, b_pitch, n0, b_n, c_lo);
-                if (full > 0) {
-                    wr.next(rr);
-                    wb.next(rb);
-                }
-                for (int64_t k = 0; k < full; ++k) {
+                wr.next(rr);
+                wb.next(rb);
+                for (int k = 0; k < full; ++k) {
                     __syncthreads();  // the last step's reads are done
                     TR::store(s0, tid, rr);
                     TB::store(s0 + P * TR::plane, tid, rb);
@@ -447,16 +505,16 @@ struct Product {
                     step(s0, acc);
                 }
             }
-        }
-        for (; c < c_hi; c += BK) {  // what is left of c, and tiles at an end that cuts a piece
-            TR::load(rr, tid, r, r_pitch, r0, r_n, c, c_hi);
-            TB::load(rb, tid, b, b_pitch, n0, b_n, c, c_hi);
-            __syncthreads();
-            TR::store(s0, tid, rr);
-            TB::store(s0 + P * TR::plane, tid, rb);
-            __syncthreads();
-            seen(s0 + P * TR::plane);
-            step(s0, acc);
+            for (; c < c_hi; c += BK) {
+                TR::load(rr, tid, r, r_pitch, r0, r_n, c, c_hi);
+                TB::load(rb, tid, b, b_pitch, n0, b_n, c, c_hi);
+                __syncthreads();
+                TR::store(s0, tid, rr);
+                TB::store(s0 + P * TR::plane, tid, rb);
+                __syncthreads();
+                seen(s0 + P * TR::plane);
+                step(s0, acc);
+            }
         }
     }
 
@@ -517,21 +575,35 @@ __device__ __forceinline__ void finish4(const GroupedArgs& a, const Item& it, co
     store4<T>((T*)a.out + row * a.cols + col, v, valid);
 }
 
-// forward (LB = ACROSS) and input gradient (LB = ALONG): a workgroup per row tile and column tile
-template <typename T, Layout LB, int BR, int BN, bool DIRECT>
-__global__ __launch_bounds__(kGlThreads, 2) void grouped_rows_kernel(GroupedArgs a) {
-    typedef Product<T, ALONG, LB, BR, BN, DIRECT> X;
-    __shared__ __attribute__((aligned(16))) typename X::E s0[X::stage];
-    __shared__ __attribute__((aligned(16))) typename X::E s1[DIRECT ? X::stage : 8];
-    const Item it = find_item<kGlThreads>(a, blockIdx.x / a.col_tiles, BR, 0, true);
-    if (it.group < 0) return;
-    const int64_t n0 = (int64_t)(blockIdx.x % a.col_tiles) * BN;
-    const int64_t r0 = it.lo + (int64_t)it.part * BR;
+// One tile of the forward (LB = ACROSS) or input gradient (LB = ALONG).
+template <typename T, Layout LB, int BR, int BN, int THREADS, bool DIRECT>
+__device__ __forceinline__ void rows_tile(const GroupedArgs& a, const Item& it, int64_t r0, int64_t n0,
+                                          typename Stage<T>::elem* s0, typename Stage<T>::elem* s1) {
+    typedef Product<T, ALONG, LB, BR, BN, THREADS, DIRECT> X;
     f32x4 acc[X::NR][X::NN] = {};
     const T* b = (const T*)a.b + (int64_t)it.group * a.b_group;
     if (it.group < a.groups)
         X::run(s0, s1, acc, (const T*)a.r, a.r_pitch, r0, it.hi, b, a.b_pitch, n0, a.cols, 0, a.cc, [](auto*) {});
     X::each(acc, [&](int ir, int in, f32x4& v) { finish4<T, LB>(a, it, b, r0 + ir, n0 + in, v); });
+}
+
+// A workgroup per row tile and column tile. At 256 rows a group's last tile of at most 128 rows costs half.
+template <typename T, Layout LB, int BR, int BN, int THREADS, bool DIRECT>
+__global__ __launch_bounds__(THREADS, 2) void grouped_rows_kernel(GroupedArgs a) {
+    typedef Product<T, ALONG, LB, BR, BN, THREADS, DIRECT> X;
+    __shared__ __attribute__((aligned(16))) typename X::E s0[X::stage];
+    __shared__ __attribute__((aligned(16))) typename X::E s1[DIRECT ? X::stage : 8];
+    const Item it = find_item<THREADS>(a, blockIdx.x / a.col_tiles, BR, 0, true);
+    if (it.group < 0) return;
+    const int64_t n0 = (int64_t)(blockIdx.x % a.col_tiles) * BN;
+    const int64_t r0 = it.lo + (int64_t)it.part * BR;
+    if constexpr (BR == 256) {
+        if (it.hi - r0 <= BR / 2) {
+            rows_tile<T, LB, BR / 2, BN, THREADS, DIRECT>(a, it, r0, n0, s0, s1);
+            return;
+        }
+    }
+    rows_tile<T, LB, BR, BN, THREADS, DIRECT>(a, it, r0, n0, s0, s1);
 }
 
 // The same for few rows a group, where the time goes into reading the weights: tiles of 32 rows and 64
@@ -541,8 +613,8 @@ template <typename T, Layout LB, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, 2) void grouped_few_rows_kernel(GroupedArgs a) {
     constexpr int BR = 32, BN = 64, NR = BR / 16, NN = BN / 16, P = Stage<T>::planes, BK = Stage<T>::bk;
     typedef typename Stage<T>::elem E;
-    typedef Tile<T, ALONG, BR, 64> TR;
-    typedef Tile<T, LB, BN, 64> TB;
+    typedef Tile<T, ALONG, BR, BK, 64> TR;
+    typedef Tile<T, LB, BN, BK, 64> TB;
     constexpr int stage = P * (TR::plane + TB::plane);
     __shared__ __attribute__((aligned(16))) E lds[WAVES * stage];
     static_assert(sizeof(E) * stage >= BR * BN * sizeof(float), "a wave's results fit its stage");
@@ -566,7 +638,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void grouped_few_rows_kernel(Grouped
             __builtin_amdgcn_wave_barrier();
         };
         auto use = [&] {
-            multiply<T, TR, TB, NR, NN>(s, s + P * TR::plane, 0, 0, acc);
+            multiply<T, TR, TB, BK, NR, NN>(s, s + P * TR::plane, 0, 0, acc);
             __builtin_amdgcn_wave_barrier();
         };
         int64_t c = c_lo;
@@ -581,13 +653,17 @@ __global__ __launch_bounds__(WAVES * 64, 2) void grouped_few_rows_kernel(Grouped
             };
             if (full > 0) get(0);
             if (full > 1) get(1);
-            for (int64_t k = 0; k < full; k += 2) {
+            int64_t k = 0;
+            for (; k + 2 <= full; k += 2) {
                 put(0);
                 if (k + 2 < full) get(0);
                 use();
-                if (k + 1 >= full) break;
                 put(1);
                 if (k + 3 < full) get(1);
+                use();
+            }
+            if (k < full) {
+                put(0);
                 use();
             }
         }
@@ -618,22 +694,22 @@ __global__ __launch_bounds__(WAVES * 64, 2) void grouped_few_rows_kernel(Grouped
 
 // weight gradient: a workgroup per chunk of a group's rows and tile of the weight. A group of one
 // chunk is written as it is; the chunks of a longer one leave fp32 slabs for the kernel below.
-template <typename T, int BR, int BN, bool DIRECT>
-__global__ __launch_bounds__(kGlThreads, 2) void grouped_wgrad_kernel(GroupedArgs a) {
-    typedef Product<T, ACROSS, ACROSS, BR, BN, DIRECT> X;
+template <typename T, int BR, int BN, int THREADS, bool DIRECT, bool BIAS>
+__global__ __launch_bounds__(THREADS, 2) void grouped_wgrad_kernel(GroupedArgs a) {
+    typedef Product<T, ACROSS, ACROSS, BR, BN, THREADS, DIRECT> X;
     __shared__ __attribute__((aligned(16))) typename X::E s0[X::stage];
     __shared__ __attribute__((aligned(16))) typename X::E s1[DIRECT ? X::stage : 8];
     const int tiles = a.row_tiles * a.col_tiles;
     const int64_t id = blockIdx.x / tiles;
     const int tile = blockIdx.x % tiles;
-    const Item it = find_item<kGlThreads>(a, id, a.chunk, 1, false);
+    const Item it = find_item<THREADS>(a, id, a.chunk, 1, false);
     if (it.group < 0) return;
     const int64_t r0 = (int64_t)(tile / a.col_tiles) * BR, n0 = (int64_t)(tile % a.col_tiles) * BN;
     const int64_t c_lo = it.lo + (int64_t)it.part * a.chunk;
     const int64_t c_hi = c_lo + a.chunk < it.hi ? c_lo + a.chunk : it.hi;
     f32x4 acc[X::NR][X::NN] = {};
     float col_sum[8] = {};  // of the columns of this thread's pieces: the same in every piece
-    const bool want_b = a.dbias && r0 == 0;
+    const bool want_b = BIAS && r0 == 0;
     const T* r = (const T*)a.r;
     const T* b = (const T*)a.b;
     X::run(s0, s1, acc, r, a.r_pitch, r0, a.out_rows, b, a.b_pitch, n0, a.cols, c_lo, c_hi, [&](auto* stage) {
@@ -655,7 +731,7 @@ __global__ __launch_bounds__(kGlThreads, 2) void grouped_wgrad_kernel(GroupedArg
         }
     });
     const int64_t size = (int64_t)a.out_rows * a.cols;
-    const int64_t slab = size + (a.dbias ? a.cols : 0);
+    const int64_t slab = size + (BIAS ? a.cols : 0);
     float* part = it.parts > 1 ? a.slabs + id * slab : nullptr;
     X::each(acc, [&](int ir, int in, f32x4& v) {
         const int64_t row = r0 + ir, col = n0 + in;
@@ -674,9 +750,10 @@ __global__ __launch_bounds__(kGlThreads, 2) void grouped_wgrad_kernel(GroupedArg
         if (part) store4<float>(part + row * a.cols + col, v, valid);
         else store4<T>((T*)a.out + (int64_t)it.group * size + row * a.cols + col, v, valid);
     });
+    if constexpr (!BIAS) return;
     if (!want_b) return;
     // the threads whose pieces have the same columns, in order
-    constexpr int teams = kGlThreads / (BN / 8);
+    constexpr int teams = THREADS / (BN / 8);
     float* sums = reinterpret_cast<float*>(s0);
     static_assert(sizeof(s0) >= teams * BN * sizeof(float), "the column sums fit the stage");
     __syncthreads();
@@ -684,7 +761,7 @@ __global__ __launch_bounds__(kGlThreads, 2) void grouped_wgrad_kernel(GroupedArg
 #pragma unroll
     for (int k = 0; k < 8; ++k) sums[team * BN + c8 + k] = col_sum[k];
     __syncthreads();
-    for (int c = threadIdx.x; c < BN && n0 + c < a.cols; c += kGlThreads) {
+    for (int c = threadIdx.x; c < BN && n0 + c < a.cols; c += THREADS) {
         float s = sums[c];
         for (int q = 1; q < teams; ++q) s += sums[q * BN + c];
         if constexpr (sizeof(T) == 4) {  // an infinity's pieces are not numbers
@@ -723,12 +800,34 @@ __global__ __launch_bounds__(kGlThreads) void grouped_slabs_kernel(GroupedArgs a
     const float* p = a.slabs + s_first * slab;
     parts = min(parts, a.items - s_first);  // short only where ptr decreases and groups overlap
     if (parts < 1) return;
-    for (int64_t e = (int64_t)(blockIdx.x % pieces) * kGlThreads + threadIdx.x; e < slab;
-         e += (int64_t)pieces * kGlThreads) {
-        float s = p[e];
-        for (int k = 1; k < parts; ++k) s += p[k * slab + e];
-        if (e < size) ((T*)a.out)[(int64_t)g * size + e] = (T)s;
-        else ((T*)a.dbias)[(int64_t)g * a.cols + e - size] = (T)s;
+    for (int64_t e = ((int64_t)(blockIdx.x % pieces) * kGlThreads + threadIdx.x) * 4; e < slab;
+         e += (int64_t)pieces * kGlThreads * 4) {
+        const int valid = slab - e < 4 ? (int)(slab - e) : 4;
+        f32x4 s = {};
+        int64_t k = 0;
+        if (valid == 4) {
+            for (; k + 8 <= parts; k += 8) {  // eight slabs on their way at once, added in order
+                f32x4 v[8];
+#pragma unroll
+                for (int q = 0; q < 8; ++q) __builtin_memcpy(&v[q], p + (k + q) * slab + e, 16);
+#pragma unroll
+                for (int q = 0; q < 8; ++q) s += v[q];
+            }
+        }
+        for (; k < parts; ++k)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (q < valid) s[q] += p[k * slab + e + q];
+        if (e + 4 <= size) {
+            store4<T>((T*)a.out + (int64_t)g * size + e, s, 4);
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                if (q >= valid) break;
+                if (e + q < size) ((T*)a.out)[(int64_t)g * size + e + q] = (T)s[q];
+                else ((T*)a.dbias)[(int64_t)g * a.cols + e + q - size] = (T)s[q];
+            }
+        }
     }
 }
 
@@ -736,6 +835,14 @@ __global__ __launch_bounds__(kGlThreads) void grouped_slabs_kernel(GroupedArgs a
 // host
 // ---------------------------------------------------------------------------------------
 constexpr int kTile = 128;
+// Tiles of 256 x 256 read half as many bytes a product as tiles of 128 x 128, which the CUs' 64 bytes a
+// clock from L2 hold to half the matrix rate; but a CU has one at a time, so that they need rounds
+// enough: bf16, us for forward / input / weight gradient with 128 and 256:
+//   32768 rows, 32 groups, 2048 x 4096   745 / 650 / 896    591 / 582 / 720
+//   32768 rows, 128 groups, 1024 x 2048  245 / 243 / 466    239 / 223 / 392
+//   16384 rows, 4 groups, 1024 x 1024     63 /  63 /  92     67 /  65 /  97
+//   8192 rows, 8 groups, 512 x 2048       36 /  36 /  65     46 /  51 /  72
+constexpr int64_t kBigTiles = 512;
 constexpr int kFewRows = 32;  // rows a group on average, up to which grouped_few_rows_kernel runs
 
 // Rows of a chunk of the weight gradient: whole groups where the weight alone has tiles enough to
@@ -763,8 +870,9 @@ int32_t check_grouped(int64_t rows, int64_t groups, int64_t k, int64_t n, int32_
 // operands that go straight to LDS: 16-bit, their rows and groups at multiples of 16 bytes
 template <typename T>
 bool direct_ok(const GroupedArgs& a) {
+    constexpr int64_t reach = 1 << 20;  // a lane's offset within a tile of 256 rows fits 32 bits
     return sizeof(T) == 2 && aligned16(a.r) && aligned16(a.b) && a.r_pitch % 8 == 0 && a.b_pitch % 8 == 0 &&
-           a.b_group % 8 == 0;
+           a.b_group % 8 == 0 && a.r_pitch <= reach && a.b_pitch <= reach;
 }
 
 template <typename T, Layout LB, int WAVES>
@@ -772,15 +880,25 @@ void launch_few(GroupedArgs a, unsigned blocks, hipStream_t strm) {
     hipLaunchKernelGGL((grouped_few_rows_kernel<T, LB, WAVES>), dim3(blocks), dim3(WAVES * 64), 0, strm, a);
 }
 
-template <typename T, Layout LB, bool DIRECT>
+template <typename T, Layout LB, int TILE, int THREADS, bool DIRECT>
 void launch_rows(GroupedArgs a, unsigned blocks, hipStream_t strm) {
-    hipLaunchKernelGGL((grouped_rows_kernel<T, LB, kTile, kTile, DIRECT>), dim3(blocks), dim3(kGlThreads), 0, strm, a);
+    hipLaunchKernelGGL((grouped_rows_kernel<T, LB, TILE, TILE, THREADS, DIRECT>), dim3(blocks), dim3(THREADS), 0, strm,
+                       a);
 }
+
+// columns that tiles of 256 cover without much more padding than tiles of 128
+bool big_cols(int64_t n) { return n % 256 == 0 || n % 256 > 128 || n >= 1024; }
 
 template <typename T, Layout LB>
 int32_t rows_product(GroupedArgs a, hipStream_t strm) {
     const bool few = a.rows <= (int64_t)kFewRows * a.groups;
-    const int br = few ? 32 : kTile, bn = few ? 64 : kTile;
+    bool direct = false, big = false;
+    if constexpr (sizeof(T) == 2) {
+        direct = !few && direct_ok<T>(a);
+        big = direct && big_cols(a.cols) && a.rows >= 256 * (int64_t)a.groups &&
+              a.rows / 256 * ((a.cols + 255) / 256) >= kBigTiles;
+    }
+    const int br = few ? 32 : big ? 256 : kTile, bn = few ? 64 : big ? 256 : kTile;
     a.col_tiles = (a.cols + bn - 1) / bn;
     const int64_t blocks = (a.rows / br + a.groups + 2) * a.col_tiles;
     if (blocks > INT32_MAX) return unsupported("grouped linear: more than 2^31 tiles");
@@ -790,14 +908,12 @@ int32_t rows_product(GroupedArgs a, hipStream_t strm) {
         const int64_t busy = std::min<int64_t>(a.rows, a.rows / br + a.groups) * a.col_tiles;
         if (busy < 512) launch_few<T, LB, 8>(a, (unsigned)blocks, strm);
         else launch_few<T, LB, 4>(a, (unsigned)blocks, strm);
+    } else if constexpr (sizeof(T) == 2) {
+        if (big) launch_rows<T, LB, 256, 512, true>(a, (unsigned)blocks, strm);
+        else if (direct) launch_rows<T, LB, kTile, 256, true>(a, (unsigned)blocks, strm);
+        else launch_rows<T, LB, kTile, 256, false>(a, (unsigned)blocks, strm);
     } else {
-        if constexpr (sizeof(T) == 2) {
-            if (direct_ok<T>(a)) {
-                launch_rows<T, LB, true>(a, (unsigned)blocks, strm);
-                return launch_status("grouped linear: the launch failed");
-            }
-        }
-        launch_rows<T, LB, false>(a, (unsigned)blocks, strm);
+        launch_rows<T, LB, kTile, 512, false>(a, (unsigned)blocks, strm);
     }
     return launch_status("grouped linear: the launch failed");
 }
@@ -813,26 +929,39 @@ int32_t rows_by_type(const GroupedArgs& a, int32_t dtype, bool dgrad, hipStream_
     return dtype == MPGNN_BF16 ? rows_either<__bf16>(a, dgrad, strm) : rows_either<_Float16>(a, dgrad, strm);
 }
 
-template <typename T>
-int32_t wgrad_product(GroupedArgs a, hipStream_t strm) {
-    a.row_tiles = (a.out_rows + kTile - 1) / kTile;
-    a.col_tiles = (a.cols + kTile - 1) / kTile;
-    a.items = wgrad_items(a.rows, a.groups, a.chunk);
+template <typename T, int TILE, int THREADS, bool DIRECT>
+int32_t launch_wgrad(GroupedArgs a, hipStream_t strm) {
+    a.row_tiles = (a.out_rows + TILE - 1) / TILE;
+    a.col_tiles = (a.cols + TILE - 1) / TILE;
     const int64_t blocks = a.items * a.row_tiles * a.col_tiles;
     if (blocks > INT32_MAX) return unsupported("grouped linear: more than 2^31 tiles");
-    bool direct = false;
+    if (a.dbias)
+        hipLaunchKernelGGL((grouped_wgrad_kernel<T, TILE, TILE, THREADS, DIRECT, true>), dim3((unsigned)blocks),
+                           dim3(THREADS), 0, strm, a);
+    else
+        hipLaunchKernelGGL((grouped_wgrad_kernel<T, TILE, TILE, THREADS, DIRECT, false>), dim3((unsigned)blocks),
+                           dim3(THREADS), 0, strm, a);
+    return MPGNN_OK;
+}
+
+template <typename T>
+int32_t wgrad_product(GroupedArgs a, hipStream_t strm) {
+    a.items = wgrad_items(a.rows, a.groups, a.chunk);
+    int32_t st;
     if constexpr (sizeof(T) == 2) {
-        direct = direct_ok<T>(a);
-        if (direct)
-            hipLaunchKernelGGL((grouped_wgrad_kernel<T, kTile, kTile, true>), dim3((unsigned)blocks), dim3(kGlThreads),
-                               0, strm, a);
+        const bool direct = direct_ok<T>(a);
+        const int64_t tiles = (int64_t)((a.out_rows + 255) / 256) * ((a.cols + 255) / 256) * a.groups;
+        if (direct && big_cols(a.out_rows) && big_cols(a.cols) && a.rows >= 256 * (int64_t)a.groups && tiles >= kBigTiles)
+            st = launch_wgrad<T, 256, 512, true>(a, strm);
+        else if (direct) st = launch_wgrad<T, kTile, 256, true>(a, strm);
+        else st = launch_wgrad<T, kTile, 256, false>(a, strm);
+    } else {
+        st = launch_wgrad<T, kTile, 512, false>(a, strm);
     }
-    if (!direct)
-        hipLaunchKernelGGL((grouped_wgrad_kernel<T, kTile, kTile, false>), dim3((unsigned)blocks), dim3(kGlThreads), 0,
-                           strm, a);
+    if (st != MPGNN_OK) return st;
     if (a.rows > a.chunk) {
-        const int64_t slab = (int64_t)a.out_rows * a.cols + a.cols;
-        const int pieces = (int)std::min<int64_t>(64, (slab + kGlThreads * 4 - 1) / (kGlThreads * 4));
+        const int64_t slab = (int64_t)a.out_rows * a.cols + (a.dbias ? a.cols : 0);
+        const int pieces = (int)std::min<int64_t>(256, (slab + kGlThreads * 4 - 1) / (kGlThreads * 4));
         hipLaunchKernelGGL(grouped_slabs_kernel<T>, dim3((unsigned)a.groups * pieces), dim3(kGlThreads), 0, strm, a,
                            pieces);
     }

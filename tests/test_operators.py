@@ -286,6 +286,40 @@ def test_grouped_linear_against_64_bits(case, dt, biased):
         assert torch.equal(mpgnn_amd.grouped_linear(xg, wg, ptr, bg), y)
 
 
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("biased", [False, True], ids=["plain", "bias"])
+@pytest.mark.parametrize("shape", [([5000, 1, 3100, 255], 3, 64, 4096), ([300] * 5 + [0, 900, 130], 0, 1024, 4096)],
+                         ids=["rows", "weights"])
+def test_grouped_linear_large(shape, dt, biased):
+    """Sizes that fill the chip with the largest tiles (whole, halved and cut ones): rows over many
+    columns, and many weights. The 64-bit products run on the GPU."""
+    sizes, behind, k, n = shape
+    g = gen(13)
+    off = offsets(sizes)
+    rows, groups = off[-1] + behind, len(sizes)
+    x, w = rnd(g, rows, k, dtype=dt).to(DEV), rnd(g, groups, k, n, scale=k ** -0.5, dtype=dt).to(DEV)
+    b = rnd(g, groups, n, dtype=dt).to(DEV) if biased else None
+    dy = rnd(g, rows, n, dtype=dt).to(DEV)
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b) if t is not None]
+    y = mpgnn_amd.grouped_linear(leaves[0], leaves[1], torch.tensor(off, device=DEV), leaves[2] if biased else None)
+    got = [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+    for q in range(groups):
+        lo, hi = off[q], off[q + 1]
+        xg, wg, dg = x[lo:hi].double(), w[q].double(), dy[lo:hi].double()
+        bg = b[q].double() if biased else torch.zeros(n, dtype=torch.float64, device=DEV)
+        pairs = [(got[0][lo:hi], xg @ wg + bg, xg.abs() @ wg.abs() + bg.abs(), k),
+                 (got[1][lo:hi], dg @ wg.t(), dg.abs() @ wg.abs().t(), n),
+                 (got[2][q], xg.t() @ dg, xg.abs().t() @ dg.abs(), hi - lo)]
+        for a, ref, mag, length in pairs:
+            assert bool(((a.double() - ref).abs() <= gl_tol(ref, mag, length, dt)).all()), (q, length)
+        if biased:
+            ref = dg.sum(0)
+            tol = ((hi - lo) / 16 + 40) * U * dg.abs().sum(0) + half(dt) * ref.abs() + tiny(dt)
+            assert bool(((got[3][q].double() - ref).abs() <= tol).all()), q
+    if behind:
+        assert float(got[0][off[-1]:].abs().max()) == 0.0 and float(got[1][off[-1]:].abs().max()) == 0.0
+
+
 def test_grouped_linear_fp32_is_as_near_as_fp32_products():
     """The split products against 64 bits, normwise: 24 accumulations of K = 128, rounding to 2^-24
     of partial sums of about the result's size each, and 2^-25 a product: below 2 sqrt(24) u."""
