@@ -8,11 +8,11 @@
 // sum over 2^28 elements keeps fp32 accuracy. Each thread adds its elements in order, then lanes,
 // waves, workgroups, always in the same order: the norm does not change from run to run.
 //
-// Two kernels per up to kClipMax tensors (the tensor table is the kernel's argument, so a captured
+// Two kernels per list of up to kClipMax tensors (the tensor table is the kernel's argument, so a captured
 // graph holds it by value): the norm kernel leaves one partial sum per workgroup, the scaling
-// kernel's workgroups each add all partials (<= 2,048 doubles from L2) and so need no counter, no
-// atomic and no third launch. A list of at most kClipSmallBytes takes one launch of one workgroup
-// that does both.
+// kernel's workgroups each add all partials (up to 2,048 doubles from L2) and so need no counter, no
+// atomic and no third launch. With more than one list, one more workgroup adds the partials of all
+// before the scaling. Tensors of at most kClipSmallBytes together take one launch of one workgroup.
 #include <algorithm>
 
 #include "num_types.h"
@@ -24,7 +24,7 @@ constexpr int kClipThreads = 256;
 constexpr int kClipMax = 120;              // tensors per launch: 3.6 KB of kernel arguments
 constexpr int kClipUnit = 16384;           // bytes of a tensor that a workgroup takes at a time
 constexpr int kClipMaxLists = 1024;
-constexpr int kClipMaxPartials = 2048;     // workgroups of all norm launches of one call
+constexpr int kClipBlocks = 2048;          // workgroups of a launch: eight per CU, all there at once
 constexpr int kClipSmallThreads = 1024;
 constexpr int64_t kClipSmallBytes = 128 * 1024;
 
@@ -174,6 +174,17 @@ __device__ __forceinline__ double join_partials(const double* partials, int n, d
     return OP::norm(block_join<OP, kClipThreads>(a, s_red));
 }
 
+// the partials of several lists into the first (each thread reads its own before any is overwritten)
+template <typename OP>
+__global__ __launch_bounds__(kClipSmallThreads) void clip_join_kernel(double* partials, int n) {
+    __shared__ double s_red[kClipSmallThreads / 64];
+    double a = 0;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < n; i += kClipSmallThreads) a = OP::join(a, partials[i]);
+    a = block_join<OP, kClipSmallThreads>(a, s_red);
+    if (threadIdx.x == 0) partials[0] = a;
+}
+
 // scale = 0: the norm alone
 template <typename OP>
 __global__ __launch_bounds__(kClipThreads) void clip_scale_kernel(ClipList L, int per_block, const double* partials,
@@ -210,12 +221,11 @@ int64_t tensor_units(const mpgnn_clip_tensor& t) {
 template <typename OP>
 int32_t clip_run(const mpgnn_clip_tensor* tensors, int32_t n, float max_norm, int32_t scale, float* norm, void* ws,
                  hipStream_t strm) {
-    int64_t bytes = 0, units = 0;
+    int64_t bytes = 0;
     int filled = 0;
     for (int k = 0; k < n; ++k) {
         filled += tensors[k].numel > 0;
         bytes += tensors[k].numel * dtype_bytes(tensors[k].dtype);
-        units += tensor_units(tensors[k]);
     }
     // the next up to kClipMax tensors with elements, from tensor `at` on; returns their units
     auto fill = [&](ClipList& L, int& at) {
@@ -242,19 +252,22 @@ int32_t clip_run(const mpgnn_clip_tensor* tensors, int32_t n, float max_norm, in
         hipLaunchKernelGGL(clip_small_kernel<OP>, dim3(1), dim3(kClipSmallThreads), 0, strm, L, max_norm, norm, scale);
         return launch_status("clip: the launch failed");
     }
-    // every launch of up to kClipMax tensors gets workgroups in proportion to its units
     const int lists = (filled + kClipMax - 1) / kClipMax;
-    const int64_t spare = kClipMaxPartials - lists;
-    const int64_t per_block = std::max<int64_t>(1, (units + spare - 1) / spare);
+    // units a workgroup
+    auto share = [](int64_t u) { return (int)((u + kClipBlocks - 1) / kClipBlocks); };
     double* partials = static_cast<double*>(ws);
     int start[kClipMaxLists];  // the first tensor of each list
     int np = 0, at = 0;
     for (int l = 0; l < lists; ++l) {
         start[l] = at;
-        const int blocks = (int)((fill(L, at) + per_block - 1) / per_block);
-        hipLaunchKernelGGL(clip_norm_kernel<OP>, dim3(blocks), dim3(kClipThreads), 0, strm, L, (int)per_block,
-                           partials + np);
+        const int64_t u = fill(L, at);
+        const int per_block = share(u), blocks = (int)((u + per_block - 1) / per_block);
+        hipLaunchKernelGGL(clip_norm_kernel<OP>, dim3(blocks), dim3(kClipThreads), 0, strm, L, per_block, partials + np);
         np += blocks;
+    }
+    if (lists > 1) {
+        hipLaunchKernelGGL(clip_join_kernel<OP>, dim3(1), dim3(kClipSmallThreads), 0, strm, partials, np);
+        np = 1;
     }
     // the lists from the last one down, each from its last unit down: what was read last is still
     // in the last-level cache
@@ -262,9 +275,9 @@ int32_t clip_run(const mpgnn_clip_tensor* tensors, int32_t n, float max_norm, in
         at = start[l];
         const int64_t u = fill(L, at);
         L.reversed = 1;
-        const int blocks = scale ? (int)((u + per_block - 1) / per_block) : 1;
-        hipLaunchKernelGGL(clip_scale_kernel<OP>, dim3(blocks), dim3(kClipThreads), 0, strm, L, (int)per_block, partials,
-                           np, max_norm, l == lists - 1 ? norm : nullptr, scale);
+        const int per_block = share(u), blocks = scale ? (int)((u + per_block - 1) / per_block) : 1;
+        hipLaunchKernelGGL(clip_scale_kernel<OP>, dim3(blocks), dim3(kClipThreads), 0, strm, L, per_block, partials, np,
+                           max_norm, l == lists - 1 ? norm : nullptr, scale);
         if (!scale) break;
     }
     return launch_status("clip: a launch failed");
@@ -277,7 +290,7 @@ extern "C" int32_t mpgnn_clip_workspace_bytes(int32_t n, int64_t* bytes) {
     using namespace mpgnn;
     if (n < 0 || !bytes) return arg_error("mpgnn_clip_workspace_bytes: negative n or bytes is null");
     if (n > kClipMax * kClipMaxLists) return unsupported("mpgnn_clip_workspace_bytes: more than 122,880 tensors");
-    *bytes = (int64_t)kClipMaxPartials * sizeof(double);
+    *bytes = (int64_t)std::max(1, (n + kClipMax - 1) / kClipMax) * kClipBlocks * (int64_t)sizeof(double);
     return MPGNN_OK;
 }
 

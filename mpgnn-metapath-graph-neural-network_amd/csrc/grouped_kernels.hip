@@ -846,10 +846,10 @@ constexpr int64_t kBigTiles = 512;
 constexpr int kFewRows = 32;  // rows a group on average, up to which grouped_few_rows_kernel runs
 
 // Rows of a chunk of the weight gradient: whole groups where the weight alone has tiles enough to
-// fill the chip, else as many rows as leave about four workgroups per CU.
+// fill the chip, else as many rows as leave about two workgroups per CU.
 int64_t wgrad_chunk(int64_t rows, int64_t groups, int64_t k, int64_t n) {
     const int64_t tiles = ((k + kTile - 1) / kTile) * ((n + kTile - 1) / kTile);
-    const int64_t want = 1024 / tiles;  // chunks over all groups
+    const int64_t want = 512 / tiles;  // chunks over all groups
     if (want <= groups || rows == 0) return std::max<int64_t>(rows, 1);
     const int64_t c = (rows + want - 1) / want;
     return std::max<int64_t>(256, (c + 63) / 64 * 64);

@@ -73,6 +73,34 @@ struct RowShape {
     static constexpr int lds = TPR > 64 ? TPR / 64 * 4 : 1;
 };
 
+// A thread's part of a row on its way from memory: the next row is asked for before the current
+// one's sums, whose barriers it does not wait for.
+template <typename T, int V, int TPR, int NV>
+struct Row {
+    typename VecOf<T, V>::type v[NV];
+
+    __device__ __forceinline__ void load(const T* p, int64_t pitch, int64_t r, int64_t rows, int t, int F) {
+        const bool live = r < rows;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * TPR + t) * V;
+            v[i] = live && c < F ? *reinterpret_cast<const typename VecOf<T, V>::type*>(p + r * pitch + c)
+                                 : typename VecOf<T, V>::type(0);
+        }
+    }
+    __device__ __forceinline__ void widen(float (&f)[NV][V]) const {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if constexpr (V == 1) {
+                f[i][0] = (float)v[i];
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; ++j) f[i][j] = (float)v[i][j];
+            }
+        }
+    }
+};
+
 template <typename T, int V, int TPR, int NV>
 __global__ __launch_bounds__(RowShape<TPR>::threads) void layer_norm_fwd_kernel(NormArgs a) {
     using S = RowShape<TPR>;
@@ -91,22 +119,15 @@ __global__ __launch_bounds__(RowShape<TPR>::threads) void layer_norm_fwd_kernel(
     const float width = (float)F;
     int turn = 0;
     const int64_t step = (int64_t)gridDim.x * S::rows;
+    Row<T, V, TPR, NV> next;
+    next.load((const T*)a.x, a.x_pitch, (int64_t)blockIdx.x * S::rows + sub, a.rows, t, F);
     // every thread of the workgroup takes part in each turn's sums; rows past the end are not touched
     for (int64_t r0 = (int64_t)blockIdx.x * S::rows; r0 < a.rows; r0 += step) {
         const int64_t r = r0 + sub;
         const bool live = r < a.rows;
-        const T* x = (const T*)a.x + r * a.x_pitch;
         float v[NV][V], s[1] = {0.0f};
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (i * TPR + t) * V;
-            if (live && c < F) {
-                load_vec<T, V>(v[i], x + c);
-            } else {
-#pragma unroll
-                for (int j = 0; j < V; ++j) v[i][j] = 0.0f;
-            }
-        }
+        next.widen(v);
+        next.load((const T*)a.x, a.x_pitch, r + step, a.rows, t, F);
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -165,37 +186,40 @@ __global__ __launch_bounds__(RowShape<TPR>::threads) void layer_norm_bwd_kernel(
     __shared__ float s_part[S::rows > 1 ? S::rows * COLS : 1];
     const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
     const int F = a.width;
-    float w[NV][V], dw[NV][V], db[NV][V], dwc[COMP ? NV : 1][V], dbc[COMP ? NV : 1][V];
+    // the weight stays in registers, but for the largest teams, whose 128 a thread have no room
+    constexpr bool KEEP = TPR < 1024;
+    float w[KEEP ? NV : 1][V], dw[NV][V], db[NV][V], dwc[COMP ? NV : 1][V], dbc[COMP ? NV : 1][V];
+    auto weight = [&](int c) { return a.w && c < F ? param_at<T>(a.w, a.w_f32, c) : 1.0f; };
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const int c = (i * TPR + t) * V + j;
-            w[i][j] = a.w && c < F ? param_at<T>(a.w, a.w_f32, c) : 1.0f;
+            if constexpr (KEEP) w[i][j] = weight((i * TPR + t) * V + j);
             dw[i][j] = db[i][j] = 0.0f;
             dwc[COMP ? i : 0][j] = dbc[COMP ? i : 0][j] = 0.0f;
         }
     const float width = (float)F;
     int turn = 0;
     const int64_t step = (int64_t)gridDim.x * S::rows;
+    Row<T, V, TPR, NV> next_x, next_dy;
+    float next_mean = 0.0f, next_rstd = 0.0f;
+    auto fetch = [&](int64_t r) {
+        next_x.load((const T*)a.x, a.x_pitch, r, a.rows, t, F);
+        next_dy.load((const T*)a.dy, a.dy_pitch, r, a.rows, t, F);
+        if (r < a.rows) {
+            next_mean = a.mean[r];
+            next_rstd = a.rstd[r];
+        }
+    };
+    fetch((int64_t)blockIdx.x * S::rows + sub);
     for (int64_t r0 = (int64_t)blockIdx.x * S::rows; r0 < a.rows; r0 += step) {
         const int64_t r = r0 + sub;
         const bool live = r < a.rows;
-        const T* x = (const T*)a.x + r * a.x_pitch;
-        const T* dy = (const T*)a.dy + r * a.dy_pitch;
-        const float mean = live ? a.mean[r] : 0.0f, rstd = live ? a.rstd[r] : 0.0f;
+        const float mean = next_mean, rstd = next_rstd;
         float xh[NV][V], g[NV][V], s[2] = {0.0f, 0.0f};
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (i * TPR + t) * V;
-            if (live && c < F) {
-                load_vec<T, V>(xh[i], x + c);
-                load_vec<T, V>(g[i], dy + c);
-            } else {
-#pragma unroll
-                for (int j = 0; j < V; ++j) xh[i][j] = g[i][j] = 0.0f;
-            }
-        }
+        next_x.widen(xh);
+        next_dy.widen(g);
+        fetch(r + step);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const bool in = live && (i * TPR + t) * V < F;
@@ -205,7 +229,7 @@ __global__ __launch_bounds__(RowShape<TPR>::threads) void layer_norm_bwd_kernel(
                 xh[i][j] = (xh[i][j] - mean) * rstd;
                 add_to<COMP>(dw[i][j], dwc[COMP ? i : 0][j], g[i][j] * xh[i][j]);
                 add_to<COMP>(db[i][j], dbc[COMP ? i : 0][j], g[i][j]);
-                g[i][j] *= w[i][j];
+                g[i][j] *= KEEP ? w[KEEP ? i : 0][j] : weight((i * TPR + t) * V + j);
                 s[0] += g[i][j];
                 s[1] = __builtin_fmaf(g[i][j], xh[i][j], s[1]);
             }
@@ -329,24 +353,24 @@ __global__ __launch_bounds__(256) void layer_norm_cols_kernel(NormArgs a, int64_
     p[(int64_t)a.width + c] = db;
 }
 
-// out[c] = sum over p of part[p][c], c over dw's columns then db's: 16 columns x 16 row slices a
+// out[c] = sum over p of part[p][c], c over dw's columns then db's: 16 columns x 64 row slices a
 // workgroup, the slices joined in order
 template <typename T>
-__global__ __launch_bounds__(256) void layer_norm_reduce_kernel(const float* part, int n_part, int32_t width, T* dw,
-                                                                 T* db, float* dw32, float* db32) {
-    __shared__ double s[16][17];
+__global__ __launch_bounds__(1024) void layer_norm_reduce_kernel(const float* part, int n_part, int32_t width, T* dw,
+                                                                  T* db, float* dw32, float* db32) {
+    __shared__ double s[64][17];
     const int64_t cols = 2 * (int64_t)width;
     const int64_t c = (int64_t)blockIdx.x * 16 + threadIdx.x % 16;
     const int slice = threadIdx.x / 16;
     double v = 0.0;
     if (c < cols) {
-#pragma unroll 4
-        for (int p = slice; p < n_part; p += 16) v += (double)part[(int64_t)p * cols + c];
+#pragma unroll 8
+        for (int p = slice; p < n_part; p += 64) v += (double)part[(int64_t)p * cols + c];
     }
     s[slice][threadIdx.x % 16] = v;
     __syncthreads();
     if (slice || c >= cols) return;
-    for (int k = 1; k < 16; ++k) v += s[k][threadIdx.x % 16];
+    for (int k = 1; k < 64; ++k) v += s[k][threadIdx.x % 16];
     const int64_t col = c < width ? c : c - width;
     T* o = c < width ? dw : db;
     float* o32 = c < width ? dw32 : db32;
@@ -354,7 +378,9 @@ __global__ __launch_bounds__(256) void layer_norm_reduce_kernel(const float* par
     if (o32) o32[col] = (float)v;
 }
 
-constexpr int kNormPartials = 512;   // workgroups (and partial rows) of a backward
+// Workgroups, and with them partial rows, of a backward: eight per CU as long as the partial rows, written
+// and read once in fp32, are at most a tenth of the traffic of x, dy and dx.
+int64_t norm_partials(int64_t rows, int eb) { return std::max<int64_t>(256, std::min<int64_t>(2048, rows * eb / 54)); }
 
 template <typename T, int V, int TPR, int NV>
 void launch_rows(const NormArgs& a, bool bwd, int max_blocks, hipStream_t strm) {
@@ -388,8 +414,6 @@ bool vec_ok(const NormArgs& a, int eb) {
            aligned16(a.out);
 }
 
-int64_t norm_partials(int64_t rows) { return std::min<int64_t>(rows, kNormPartials); }
-
 template <typename T>
 int32_t norm_fwd(const NormArgs& a, hipStream_t strm) {
     constexpr int max_blocks = 256 * 16;
@@ -404,20 +428,21 @@ int32_t norm_fwd(const NormArgs& a, hipStream_t strm) {
 template <typename T>
 int32_t norm_bwd(const NormArgs& a, void* dw, void* db, hipStream_t strm) {
     int parts = 0;
+    const int max_parts = (int)norm_partials(a.rows, sizeof(T));
     const int V = vec_ok(a, sizeof(T)) ? 16 / (int)sizeof(T) : 1;
     const int vecs = (a.width + V - 1) / V;
     const int rows_per = vecs <= 16 ? 16 : vecs <= 32 ? 8 : vecs <= 128 ? 4 : 1;
     if (a.rows == 0) {  // no partial rows: the parameters' gradients are zero
     } else if (vecs <= 2048) {
-        parts = (int)std::min<int64_t>(kNormPartials, (a.rows + rows_per - 1) / rows_per);
-        if (V == 1) launch_by_width<T, 1>(a, true, kNormPartials, strm);
-        else launch_by_width<T, 16 / sizeof(T)>(a, true, kNormPartials, strm);
+        parts = (int)std::min<int64_t>(max_parts, (a.rows + rows_per - 1) / rows_per);
+        if (V == 1) launch_by_width<T, 1>(a, true, max_parts, strm);
+        else launch_by_width<T, 16 / sizeof(T)>(a, true, max_parts, strm);
     } else {
         if (a.out)
             hipLaunchKernelGGL(layer_norm_bwd_wide_kernel<T>, dim3((unsigned)std::min<int64_t>(a.rows, 1024)),
                                dim3(kWide), 0, strm, a);
         if (a.part) {
-            const int64_t slice = (a.rows + kNormPartials - 1) / kNormPartials;
+            const int64_t slice = (a.rows + max_parts - 1) / max_parts;
             parts = (int)((a.rows + slice - 1) / slice);
             hipLaunchKernelGGL(layer_norm_cols_kernel<T>, dim3((a.width + 255) / 256, parts), dim3(256), 0, strm, a,
                                slice);
@@ -428,7 +453,7 @@ int32_t norm_bwd(const NormArgs& a, void* dw, void* db, hipStream_t strm) {
         T* b = a.w_f32 ? nullptr : (T*)db;
         float* w32 = a.w_f32 ? (float*)dw : nullptr;
         float* b32 = a.w_f32 ? (float*)db : nullptr;
-        hipLaunchKernelGGL(layer_norm_reduce_kernel<T>, dim3((unsigned)((2 * (int64_t)a.width + 15) / 16)), dim3(256), 0,
+        hipLaunchKernelGGL(layer_norm_reduce_kernel<T>, dim3((unsigned)((2 * (int64_t)a.width + 15) / 16)), dim3(1024), 0,
                            strm, a.part, parts, a.width, w, b, w32, b32);
     }
     return launch_status("mpgnn_layer_norm_bwd: a launch failed");
@@ -468,7 +493,7 @@ extern "C" int32_t mpgnn_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t wi
     using namespace mpgnn;
     if (rows < 0 || width <= 0 || !bytes)
         return arg_error("mpgnn_layer_norm_bwd_workspace_bytes: bad shape or bytes is null");
-    *bytes = norm_partials(rows) * 2 * width * (int64_t)sizeof(float);
+    *bytes = std::min<int64_t>(rows, norm_partials(rows, 4)) * 2 * width * (int64_t)sizeof(float);
     return MPGNN_OK;
 }
 

@@ -16,11 +16,13 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 
 import torch
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
-from ._lib import BF16, F16, F32, NORM_2, NORM_INF, ClipTensor, check, lib
+from ._lib import BF16, F16, F32, NORM_2, NORM_INF, check, lib
 from .functional import _ptr, _stream_of
 
 __all__ = ["layer_norm", "grouped_linear", "clip_by_global_norm", "clip_grad_norm_"]
@@ -263,9 +265,12 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, group_ptr: torch.Tenso
 # ---------------------------------------------------------------------------------------
 # global norm and clipping
 # ---------------------------------------------------------------------------------------
+_CLIP_RECORD = struct.Struct("=QQqii")  # mpgnn_clip_tensor
+
+
 def _clip(grads, outs, max_norm, norm_type) -> torch.Tensor:
     """The norm of ``grads`` (one device, contiguous); ``outs``: where the scaled tensors go, or None."""
-    if norm_type == 2 or norm_type == 2.0:
+    if norm_type == 2.0:
         kind = NORM_2
     elif norm_type == math.inf:
         kind = NORM_INF
@@ -273,37 +278,37 @@ def _clip(grads, outs, max_norm, norm_type) -> torch.Tensor:
         raise ValueError(f"norm_type must be 2 or inf, got {norm_type!r}")
     n = len(grads)
     device = grads[0].device
-    arr = (ClipTensor * n)()
-    for k in range(n):
-        g = grads[k]
-        a = arr[k]
-        a.grad = g.data_ptr()
-        a.numel = g.numel()
-        a.dtype = _DTYPE[g.dtype]
-        if outs is not None:
-            a.out = outs[k].data_ptr()
-    norm = torch.empty((), dtype=torch.float32, device=device)
+    # the records packed at once: hundreds of tensors a step make this loop the call's host time
+    pack = _CLIP_RECORD.pack
+    if outs is None:
+        table = b"".join([pack(g.data_ptr(), 0, g.numel(), _DTYPE[g.dtype], 0) for g in grads])
+    elif outs is grads:
+        table = b"".join([pack(p, p, g.numel(), _DTYPE[g.dtype], 0) for g in grads for p in (g.data_ptr(),)])
+    else:
+        table = b"".join([pack(g.data_ptr(), o.data_ptr(), g.numel(), _DTYPE[g.dtype], 0)
+                          for g, o in zip(grads, outs)])
     nbytes = ctypes.c_int64()
-    check(lib.mpgnn_clip_workspace_bytes(n, ctypes.byref(nbytes)), "mpgnn_clip_workspace_bytes")
+    st = lib.mpgnn_clip_workspace_bytes(n, ctypes.byref(nbytes))
+    if st:
+        check(st, "mpgnn_clip_workspace_bytes")
     ws = torch.empty(nbytes.value, dtype=torch.uint8, device=device)
+    norm = torch.empty((), dtype=torch.float32, device=device)
     with _on(device) as stream:
-        st = lib.mpgnn_clip_by_global_norm(ctypes.addressof(arr), n, kind, max_norm, norm.data_ptr(), ws.data_ptr(),
-                                           stream)
+        st = lib.mpgnn_clip_by_global_norm(table, n, kind, max_norm, norm.data_ptr(), ws.data_ptr(), stream)
     if st:
         check(st, "mpgnn_clip_by_global_norm")
+    if outs is not None:
+        increment_version(outs)  # written behind autograd's back, as any in-place operator counts
     return norm
 
 
 def _check_list(tensors, what):
-    if not tensors:
-        return
     device = tensors[0].device
     for t in tensors:
-        if t.dtype not in _DTYPE or not t.is_cuda or t.layout is not torch.strided:
+        if not (t.is_cuda and t.dtype in _DTYPE and t.layout is torch.strided and t.device == device):
             if t.layout is not torch.strided:
                 raise TypeError(f"mpgnn_amd: {what} must be dense, got {t.layout}")
             _require(t, what)
-        if t.device != device:
             raise RuntimeError(f"{what} are on several devices: {device} and {t.device}")
 
 
@@ -317,9 +322,11 @@ def _check_max_norm(max_norm) -> float:
 def _distinct(tensors, what):
     """Each tensor with elements starts at an address of its own: scaled in place twice, one would
     be scaled by the factor's square."""
-    ptrs = [t.data_ptr() for t in tensors if t.numel()]
-    if len(set(ptrs)) != len(ptrs):
-        raise ValueError(f"{what} holds one tensor twice")
+    ptrs = [t.data_ptr() for t in tensors]
+    if len(set(ptrs)) != len(ptrs):  # empty tensors may share one
+        ptrs = [t.data_ptr() for t in tensors if t.numel()]
+        if len(set(ptrs)) != len(ptrs):
+            raise ValueError(f"{what} holds one tensor twice")
 
 
 def clip_by_global_norm(tensors, max_norm: float, norm_type: float = 2.0, out=None):
@@ -331,21 +338,21 @@ def clip_by_global_norm(tensors, max_norm: float, norm_type: float = 2.0, out=No
     The factor is computed and applied in fp32 and each product rounded once to its tensor's type. An
     infinite or NaN gradient makes the norm so, and the products what the formula gives."""
     max_norm = _check_max_norm(max_norm)
-    tensors = [t.detach() for t in tensors]
+    tensors = list(tensors)
     if not tensors:
         raise ValueError("clip_by_global_norm needs at least one tensor")
     _check_list(tensors, "tensors")
     if out is None:
         outs = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in tensors]
     else:
-        outs = [o.detach() for o in out]
+        outs = list(out)
         if len(outs) != len(tensors):
             raise ValueError(f"out has {len(outs)} tensors for {len(tensors)}")
         for o, t in zip(outs, tensors):
-            if o.shape != t.shape or o.dtype != t.dtype or o.device != t.device or not o.is_contiguous():
+            if not (o.dtype == t.dtype and o.shape == t.shape and o.device == t.device and o.is_contiguous()):
                 raise ValueError("out must hold contiguous tensors of the inputs' shapes, types and device")
         _distinct(outs, "out")
-    grads = [t if t.is_contiguous() else t.contiguous() for t in tensors]
+    grads = [t if t.is_contiguous() else t.detach().contiguous() for t in tensors]
     return _clip(grads, outs, max_norm, norm_type), outs
 
 
@@ -364,7 +371,6 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_i
     grads = [g for g in (p.grad for p in parameters) if g is not None]
     if not grads:
         return torch.tensor(0.0)
-    grads = [g.detach() for g in grads]
     _check_list(grads, "gradients")
     _distinct(grads, "the parameters' gradients")
     flat = grads
@@ -376,7 +382,7 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_i
             if any(st == 0 and n > 1 for n, st in zip(g.shape, g.stride())):
                 raise ValueError("a gradient is an expanded tensor, whose elements share memory: it cannot be scaled "
                                  "in place")
-            flat[k] = g.contiguous()
+            flat[k] = g.detach().contiguous()
     if error_if_nonfinite:
         norm = _clip(flat, None, max_norm, norm_type)
         if not math.isfinite(float(norm)):
@@ -384,6 +390,8 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_i
                                "it cannot be clipped. To disable this error and scale the gradients by the non-finite "
                                "norm anyway, set `error_if_nonfinite=False`")
     norm = _clip(flat, flat, max_norm, norm_type)
-    for k in strided:
-        grads[k].copy_(flat[k])
+    if strided:
+        with torch.no_grad():
+            for k in strided:
+                grads[k].copy_(flat[k])
     return norm
