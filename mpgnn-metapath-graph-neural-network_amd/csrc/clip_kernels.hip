@@ -4,8 +4,10 @@
 // Bound by memory: each gradient is read for the norm, read again and written for the scaling
 // (the second read comes from the 256 MB last-level cache while the list fits it).
 //
-// Squares are summed in double: no fp32 gradient's square overflows or underflows there, and a
-// sum over 2^28 elements keeps fp32 accuracy. Each thread adds its elements in order, then lanes,
+// Squares are summed in double, sixteen bytes' worth at a time from an fp32 sum of at most eight squares (a
+// conversion to double takes four times an fp32 addition's time), unless that sum leaves the range in which
+// its squares are sure to be whole: then each square is taken in double, where no fp32 value's
+// overflows or vanishes. A sum over 2^28 elements keeps fp32 accuracy. Each thread adds its elements in order, then lanes,
 // waves, workgroups, always in the same order: the norm does not change from run to run.
 //
 // Two kernels per list of up to kClipMax tensors (the tensor table is the kernel's argument, so a captured
@@ -26,7 +28,7 @@ constexpr int kClipUnit = 16384;           // bytes of a tensor that a workgroup
 constexpr int kClipMaxLists = 1024;
 constexpr int kClipBlocks = 2048;          // workgroups of a launch: eight per CU, all there at once
 constexpr int kClipSmallThreads = 1024;
-constexpr int64_t kClipSmallBytes = 128 * 1024;
+constexpr int64_t kClipSmallBytes = 32 * 1024;
 
 struct ClipList {
     int n;
@@ -41,6 +43,16 @@ struct ClipList {
 struct SumSq {
     typedef double acc;
     static __device__ __forceinline__ acc add(acc a, float v) { return __builtin_fma((double)v, (double)v, a); }
+    template <int V>
+    static __device__ __forceinline__ acc add_vec(acc a, const float (&v)[V]) {
+        float s = v[0] * v[0];
+#pragma unroll
+        for (int j = 1; j < V; ++j) s = __builtin_fmaf(v[j], v[j], s);
+        if (s > 1e-25f && s < 1e37f) return a + (double)s;  // squares below 2^-149 are below 2^-24 of s
+#pragma unroll
+        for (int j = 0; j < V; ++j) a = add(a, v[j]);
+        return a;
+    }
     static __device__ __forceinline__ acc join(acc a, acc b) { return a + b; }
     static __device__ __forceinline__ double norm(acc a) { return ::sqrt(a); }
 };
@@ -49,48 +61,77 @@ struct MaxAbs {  // a NaN anywhere stays
     typedef double acc;
     static __device__ __forceinline__ acc join(acc a, acc b) { return (b > a || b != b) ? b : a; }
     static __device__ __forceinline__ acc add(acc a, float v) { return join(a, (double)__builtin_fabsf(v)); }
+    template <int V>
+    static __device__ __forceinline__ acc add_vec(acc a, const float (&v)[V]) {
+        float m = __builtin_fabsf(v[0]);
+#pragma unroll
+        for (int j = 1; j < V; ++j) {
+            const float b = __builtin_fabsf(v[j]);
+            m = (b > m || b != b) ? b : m;
+        }
+        return join(a, (double)m);
+    }
     static __device__ __forceinline__ double norm(acc a) { return a; }
+};
+
+// A unit of a tensor: its whole vectors of 16 bytes (those of a thread asked for together), then the last
+// elements of the tensor; tensors that are not aligned to 16 bytes go element by element.
+template <typename T, int THREADS>
+struct Unit {
+    static constexpr int V = 16 / sizeof(T), U = kClipUnit / sizeof(T), N = U / (THREADS * V);
+    int64_t e0, end;
+
+    __device__ __forceinline__ Unit(int64_t numel, int64_t unit) : e0(unit * U), end(min(e0 + U, numel)) {}
+    __device__ __forceinline__ int64_t at(int i) const { return e0 + (i * THREADS + (int)threadIdx.x) * V; }
+    __device__ __forceinline__ bool whole(int i) const { return at(i) + V <= end; }
+    __device__ __forceinline__ void load(float (&v)[N][V], const T* g) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (whole(i)) load_vec<T, V>(v[i], g + at(i));
+    }
+    __device__ __forceinline__ int64_t tail() const {  // this thread's element behind the whole vectors, or end
+        const int64_t e = end - (end - e0) % V + (int)threadIdx.x;
+        return e < end ? e : end;
+    }
 };
 
 template <typename T, typename OP, int THREADS>
 __device__ __forceinline__ typename OP::acc unit_norm(const T* g, int64_t numel, int64_t unit, typename OP::acc a) {
-    constexpr int V = 16 / sizeof(T), U = kClipUnit / sizeof(T);
-    constexpr int N = U / (THREADS * V);
-    const int64_t e0 = unit * U;
-    if ((reinterpret_cast<uintptr_t>(g) & 15) == 0 && e0 + U <= numel) {
-        // the unit's loads issued together
-        float v[N][V];
+    typedef Unit<T, THREADS> X;
+    const X u(numel, unit);
+    if ((reinterpret_cast<uintptr_t>(g) & 15) == 0) {
+        float v[X::N][X::V];
+        u.load(v, g);
 #pragma unroll
-        for (int i = 0; i < N; ++i) load_vec<T, V>(v[i], g + e0 + (i * THREADS + (int)threadIdx.x) * V);
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-#pragma unroll
-            for (int j = 0; j < V; ++j) a = OP::add(a, v[i][j]);
+        for (int i = 0; i < X::N; ++i)
+            if (u.whole(i)) a = OP::template add_vec<X::V>(a, v[i]);
+        if (u.tail() < u.end) a = OP::add(a, (float)g[u.tail()]);
     } else {
-        const int64_t end = e0 + U < numel ? e0 + U : numel;
-        for (int64_t e = e0 + threadIdx.x; e < end; e += THREADS) a = OP::add(a, (float)g[e]);
+#pragma unroll 8
+        for (int64_t e = u.e0 + threadIdx.x; e < u.end; e += THREADS) a = OP::add(a, (float)g[e]);
     }
     return a;
 }
 
 template <typename T, int THREADS>
 __device__ __forceinline__ void unit_scale(const T* g, T* o, int64_t numel, int64_t unit, float c) {
-    constexpr int V = 16 / sizeof(T), U = kClipUnit / sizeof(T);
-    constexpr int N = U / (THREADS * V);
-    const int64_t e0 = unit * U;
-    if (((reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(o)) & 15) == 0 && e0 + U <= numel) {
-        float v[N][V];
+    typedef Unit<T, THREADS> X;
+    const X u(numel, unit);
+    if (((reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(o)) & 15) == 0) {
+        float v[X::N][X::V];
+        u.load(v, g);
 #pragma unroll
-        for (int i = 0; i < N; ++i) load_vec<T, V>(v[i], g + e0 + (i * THREADS + (int)threadIdx.x) * V);
+        for (int i = 0; i < X::N; ++i) {
+            if (!u.whole(i)) continue;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-#pragma unroll
-            for (int j = 0; j < V; ++j) v[i][j] *= c;
-            store_vec<T, V>(o + e0 + (i * THREADS + (int)threadIdx.x) * V, v[i]);
+            for (int j = 0; j < X::V; ++j) v[i][j] *= c;
+            store_vec<T, X::V>(o + u.at(i), v[i]);
         }
+        const int64_t e = u.tail();
+        if (e < u.end) o[e] = (T)((float)g[e] * c);
     } else {
-        const int64_t end = e0 + U < numel ? e0 + U : numel;
-        for (int64_t e = e0 + threadIdx.x; e < end; e += THREADS) o[e] = (T)((float)g[e] * c);
+#pragma unroll 8
+        for (int64_t e = u.e0 + threadIdx.x; e < u.end; e += THREADS) o[e] = (T)((float)g[e] * c);
     }
 }
 

@@ -121,15 +121,16 @@ struct Item {
 // Item `id` of the list of all groups' parts: each group has ceil(rows / size) of them, at least
 // `least`. With `rest`, the rows before ptr[0] and from ptr[G] on follow as two more groups.
 template <int THREADS>
-__device__ __forceinline__ Item find_item(const GroupedArgs& a, int64_t id, int size, int least, bool rest) {
-    __shared__ int64_t s_wave[THREADS / 64];
+__device__ __forceinline__ Item find_item(const GroupedArgs& a, int id, int size, int least, bool rest) {
+    __shared__ int s_wave[THREADS / 64];
     __shared__ Item s_item;
     const int n = a.groups + (rest ? 2 : 0);
     if (threadIdx.x == 0) s_item.group = -1;
-    int64_t base = 0;
+    int base = 0;  // parts before g0: the host launches no more than 2^31
     for (int g0 = 0; g0 < n; g0 += THREADS) {
         const int g = g0 + threadIdx.x;
-        int64_t lo = 0, hi = 0, parts = 0;
+        int64_t lo = 0, hi = 0;
+        int parts = 0;
         if (g < a.groups) {
             lo = ptr_at(a, g);
             hi = ptr_at(a, g + 1);
@@ -141,29 +142,29 @@ __device__ __forceinline__ Item find_item(const GroupedArgs& a, int64_t id, int 
             hi = ptr_at(a, 0);
         }
         if (g < n) {
-            parts = (hi - lo + size - 1) / size;
+            parts = (int)((unsigned long long)(hi - lo + size - 1) / (unsigned)size);
             if (g < a.groups && parts < least) parts = least;
         }
-        int64_t sum = parts;  // inclusive scan over the wave
+        int sum = parts;  // inclusive scan over the wave
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
-            const int64_t v = __shfl_up(sum, d, 64);
+            const int v = __shfl_up(sum, d, 64);
             if ((int)(threadIdx.x % 64) >= d) sum += v;
         }
         if (threadIdx.x % 64 == 63) s_wave[threadIdx.x / 64] = sum;
         __syncthreads();
-        int64_t before = base;
+        int before = base;
+#pragma unroll
         for (int w = 0; w < THREADS / 64; ++w) {
             if (w < (int)(threadIdx.x / 64)) before += s_wave[w];
             base += s_wave[w];
         }
-        const int64_t first = before + sum - parts;
+        const int first = before + sum - parts;
         if (id >= first && id < first + parts)
-            s_item = Item{g < a.groups ? g : a.groups, (int)(id - first), (int)parts, lo, hi};
+            s_item = Item{g < a.groups ? g : a.groups, id - first, parts, lo, hi};
         __syncthreads();
         if (base > id) break;
     }
-    __syncthreads();
     Item it = s_item;  // the same in every lane: into scalar registers
     it.group = __builtin_amdgcn_readfirstlane(it.group);
     it.part = __builtin_amdgcn_readfirstlane(it.part);
@@ -246,16 +247,22 @@ struct Tile {
             idx = id % (IDX / 8) * 8;
         }
     }
-    static_assert(L == ALONG || IDX % 64 == 0, "ACROSS: the four 32-byte blocks of 128 bytes trade places");
+    // ACROSS: how the 32-byte blocks of row c trade places. A transposed read takes rows c to c + 3 (and 4
+    // on) for its first 16 lanes and c + 8 to c + 11 for the next: these eight lie in eight places of the
+    // 256 bytes that the LDS serves in a cycle.
+    static_assert(L == ALONG || IDX % 128 == 0 || IDX == 64, "the blocks of a row are four or eights");
+    static __device__ __forceinline__ int trade(int c) {
+        return IDX == 64 ? (c >> 1 & 1) | (c >> 2 & 2) : (c & 3) | (c >> 1 & 4);
+    }
     static __device__ __forceinline__ int turn(int idx) { return BK == 64 ? idx & 7 : (idx >> 1) & 3; }  // ALONG
     static __device__ __forceinline__ int offset(int idx, int c) {
         if constexpr (L == ALONG) return idx * BK + ((c / 8) ^ turn(idx)) * 8 + c % 8;
-        else return c * IDX + ((idx / 16) ^ (c & 3)) * 16 + idx % 16;
+        else return c * IDX + ((idx / 16) ^ trade(c)) * 16 + idx % 16;
     }
     // The fragment of indices i0 + i .. + 15 and c .. c + 31, of which a lane has 8 values of c from c + 8 *
     // (lane / 16) on, of index i0 + i + lane % 16: at(i0) is the lane's place for i = c = 0, and i and c,
-    // constants in the unrolled loops, change bits of it that it leaves alone (i0: a multiple of
-    // 64, or of 32 with i < 32).
+    // constants in the unrolled loops, change bits of it that it leaves alone (i < 128, and i0 a multiple
+    // of a power of two above i; c a multiple of 32).
     static __device__ __forceinline__ unsigned at(int i0) {
         const int lane = threadIdx.x % 64;
         return L == ALONG ? offset(i0 + lane % 16, lane / 16 * 8)
@@ -265,8 +272,8 @@ struct Tile {
         if constexpr (L == ALONG) {
             return *reinterpret_cast<const typename Frag<E>::type*>(lds + (at ^ c) + i * BK);
         } else {
-            const E* p = lds + (at ^ (i & 48)) + i / 64 * 64 + c * IDX;
-            return read_across<typename Frag<E>::type>(p, p + 4 * IDX);
+            const E* p = lds + (at ^ i) + c * IDX;
+            return read_across<typename Frag<E>::type>(p, p + 4 * IDX);  // c + 4 trades as c does
         }
     }
     // the tile of `p` whose indices start at i0 (of i_n) and whose c at c0 (of c_n); outside: zero
@@ -358,22 +365,24 @@ struct Tile {
                     at[n] = (unsigned)((idx < end ? idx : end - 1) * (int)pitch + ((slot % (BK / 8)) ^ turn(idx)) * 8) * 2;
                 } else {
                     const int c = slot / (IDX / 8), s = slot % (IDX / 8);
-                    const int idx = ((s / 2) ^ (c & 3)) * 16 + s % 2 * 8;
+                    const int idx = ((s / 2) ^ trade(c)) * 16 + s % 2 * 8;
                     at[n] = (unsigned)(c * (int)pitch + (idx < end ? idx : end - 8)) * 2;
                 }
             }
             base = L == ALONG ? p + i0 * pitch + c0 : p + c0 * pitch + i0;
             step = L == ALONG ? BK : BK * pitch;
         }
-        // (written out, as the compiler would wait for every load before it reads any stage)
+        // (Written out, as the compiler would wait for every load before it reads any stage. The wait states are the
+        // ones that m0 needs before a load to LDS and that a scalar from a vector lane needs before a load.)
         __device__ __forceinline__ void next(E* lds) {
             typedef __attribute__((address_space(3))) E* lptr;
-            const unsigned to = (unsigned)(unsigned long long)(lptr)lds + wave_at;
+            const unsigned to = __builtin_amdgcn_readfirstlane((unsigned)(unsigned long long)(lptr)lds + wave_at);
+            const int64_t from = scalar((int64_t)base);
 #pragma unroll
             for (int n = 0; n < chunks; ++n)
-                asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1"
+                asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1"
                              :
-                             : "v"(at[n]), "s"(base), "s"(to + n * THREADS * 16)
+                             : "v"(at[n]), "s"(from), "s"(to + n * THREADS * 16)
                              : "memory");
             base += step;
         }
@@ -389,11 +398,11 @@ __device__ __forceinline__ void multiply(const typename Stage<T>::elem* lr, cons
                                          int n0, f32x4 (&acc)[NR][NN]) {
     typedef typename Stage<T>::elem E;
     constexpr int P = Stage<T>::planes;
-    // kept from being found once for every fragment and stage: more registers than there are
     unsigned at_r = TR::at(r0), at_b = TB::at(n0);
-    asm volatile("" : "+v"(at_r), "+v"(at_b));
 #pragma unroll
     for (int c = 0; c < BK; c += 32) {
+        // kept from being found once for every fragment and stage: more registers than there are
+        asm volatile("" : "+v"(at_r), "+v"(at_b));
         typename Frag<E>::type fb[P][NN];
 #pragma unroll
         for (int p = 0; p < P; ++p)
@@ -487,16 +496,19 @@ struct Product {
             }
         } else {
             Raw<T> rr[TR::chunks], rb[TB::chunks];
+            auto put = [&] {
+                __syncthreads();  // the last step's reads are done
+                TR::store(s0, tid, rr);
+                TB::store(s0 + P * TR::plane, tid, rb);
+                __syncthreads();
+            };
             if (full > 0) {
                 typename TR::Walk wr(tid, r, r_pitch, r0, r_n, c_lo);
                 typename TB::Walk wb(tid, b, b_pitch, n0, b_n, c_lo);
                 wr.next(rr);
                 wb.next(rb);
                 for (int k = 0; k < full; ++k) {
-                    __syncthreads();  // the last step's reads are done
-                    TR::store(s0, tid, rr);
-                    TB::store(s0 + P * TR::plane, tid, rb);
-                    __syncthreads();
+                    put();
                     if (k + 1 < full) {
                         wr.next(rr);
                         wb.next(rb);
@@ -508,25 +520,19 @@ struct Product {
             for (; c < c_hi; c += BK) {
                 TR::load(rr, tid, r, r_pitch, r0, r_n, c, c_hi);
                 TB::load(rb, tid, b, b_pitch, n0, b_n, c, c_hi);
-                __syncthreads();
-                TR::store(s0, tid, rr);
-                TB::store(s0 + P * TR::plane, tid, rb);
-                __syncthreads();
+                put();
                 seen(s0 + P * TR::plane);
                 step(s0, acc);
             }
         }
     }
 
-    // f(row, column, its four results) for each quadruple that this lane holds
-    template <typename F>
-    static __device__ __forceinline__ void each(f32x4 (&acc)[NR][NN], F&& f) {
-        const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
-        const int r0 = wave / waves_n * WR, n0 = wave % waves_n * WN;
-#pragma unroll
-        for (int i = 0; i < NR; ++i)
-#pragma unroll
-            for (int j = 0; j < NN; ++j) f(r0 + i * 16 + lane % 16, n0 + j * 16 + lane / 16 * 4, acc[i][j]);
+    // this lane's results: four columns from col(j) on of row row(i)
+    static __device__ __forceinline__ int row(int i) {
+        return threadIdx.x / 64 / waves_n * WR + i * 16 + threadIdx.x % 16;
+    }
+    static __device__ __forceinline__ int col(int j) {
+        return threadIdx.x / 64 % waves_n * WN + j * 16 + threadIdx.x % 64 / 16 * 4;
     }
 };
 
@@ -546,33 +552,52 @@ __device__ __forceinline__ void store4(T* p, const f32x4& v, int valid) {
     }
 }
 
-// Four results of the forward or input gradient: what is not finite in fp32 again from the operands,
-// the bias, and the rounding to T.
-template <typename T, Layout LB>
-__device__ __forceinline__ void finish4(const GroupedArgs& a, const Item& it, const T* b, int64_t row, int64_t col,
-                                        f32x4& v) {
-    if (row >= it.hi || col >= a.cols) return;
-    const int valid = a.cols - col < 4 ? (int)(a.cols - col) : 4;
-    const bool owned = it.group < a.groups;
-    if constexpr (sizeof(T) == 4) {
-        const T* r = (const T*)a.r;
+// Is a result of this wave not finite? (0 * v is not a number then.) The split of an fp32 infinity or NaN
+// gives none of the results that a sum of products has, nor does one that overflows in its pieces.
+template <int NR, int NN>
+__device__ __forceinline__ bool any_lost(const f32x4 (&acc)[NR][NN]) {
+    float s = 0.0f;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            if (finite(v[k]) || k >= valid || !owned) continue;
-            float s = 0.0f;
-            for (int c = 0; c < a.cc; ++c)
-                s = __builtin_fmaf(r[row * a.r_pitch + c], LB == ALONG ? b[(col + k) * a.b_pitch + c]
-                                                                       : b[c * a.b_pitch + col + k], s);
-            v[k] = s;
-        }
-    }
-    if (owned && a.bias) {
-        const T* bias = (const T*)a.bias + (int64_t)it.group * a.cols;
+    for (int i = 0; i < NR; ++i)
+#pragma unroll
+        for (int j = 0; j < NN; ++j)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s = __builtin_fmaf(acc[i][j][k], 0.0f, s);
+    return __any(!(s == 0.0f));
+}
+
+// One result of the forward or input gradient from the operands.
+template <typename T, Layout LB>
+__device__ float product_again(const GroupedArgs& a, const T* b, int64_t row, int64_t col) {
+    const T* r = (const T*)a.r + row * a.r_pitch;
+    float s = 0.0f;
+    for (int c = 0; c < a.cc; ++c)
+        s = __builtin_fmaf((float)r[c], (float)(LB == ALONG ? b[col * a.b_pitch + c] : b[c * a.b_pitch + col]), s);
+    return s;
+}
+
+__device__ __forceinline__ int valid4(int64_t col, int64_t cols) {
+    return col >= cols ? 0 : cols - col < 4 ? (int)(cols - col) : 4;
+}
+
+// the bias of four columns, zeros where there is none
+template <typename T>
+__device__ __forceinline__ f32x4 bias4(const GroupedArgs& a, const Item& it, int64_t col) {
+    f32x4 v = {};
+    const int valid = valid4(col, a.cols);
+    if (!a.bias || it.group >= a.groups || !valid) return v;
+    const T* p = (const T*)a.bias + (int64_t)it.group * a.cols + col;
+    if (valid == 4) {
+        T e[4];
+        __builtin_memcpy(e, p, sizeof(e));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = (float)e[k];
+    } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-            if (k < valid) v[k] += (float)bias[col + k];
+            if (k < valid) v[k] = (float)p[k];
     }
-    store4<T>((T*)a.out + row * a.cols + col, v, valid);
+    return v;
 }
 
 // One tile of the forward (LB = ACROSS) or input gradient (LB = ALONG).
@@ -584,7 +609,32 @@ __device__ __forceinline__ void rows_tile(const GroupedArgs& a, const Item& it, 
     const T* b = (const T*)a.b + (int64_t)it.group * a.b_group;
     if (it.group < a.groups)
         X::run(s0, s1, acc, (const T*)a.r, a.r_pitch, r0, it.hi, b, a.b_pitch, n0, a.cols, 0, a.cc, [](auto*) {});
-    X::each(acc, [&](int ir, int in, f32x4& v) { finish4<T, LB>(a, it, b, r0 + ir, n0 + in, v); });
+    if constexpr (sizeof(T) == 4) {
+        if (it.group < a.groups && any_lost(acc)) {
+#pragma unroll
+            for (int i = 0; i < X::NR; ++i)
+#pragma unroll
+                for (int j = 0; j < X::NN; ++j)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (r0 + X::row(i) < it.hi && n0 + X::col(j) + k < a.cols && !finite(acc[i][j][k]))
+                            acc[i][j][k] = product_again<T, LB>(a, b, r0 + X::row(i), n0 + X::col(j) + k);
+        }
+    }
+    f32x4 add[X::NN];
+#pragma unroll
+    for (int j = 0; j < X::NN; ++j) add[j] = bias4<T>(a, it, n0 + X::col(j));
+#pragma unroll
+    for (int i = 0; i < X::NR; ++i) {
+        const int64_t row = r0 + X::row(i);
+        if (row >= it.hi) continue;
+#pragma unroll
+        for (int j = 0; j < X::NN; ++j) {
+            const int64_t col = n0 + X::col(j);
+            const int valid = valid4(col, a.cols);
+            if (valid) store4<T>((T*)a.out + row * a.cols + col, acc[i][j] + add[j], valid);
+        }
+    }
 }
 
 // A workgroup per row tile and column tile. At 256 rows a group's last tile of at most 128 rows costs half.
@@ -688,7 +738,15 @@ __global__ __launch_bounds__(WAVES * 64, 2) void grouped_few_rows_kernel(Grouped
         f32x4 v = {};
         for (int w = 0; w < WAVES; ++w)
             v += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + w * stage) + ir * BN + in);
-        finish4<T, LB>(a, it, b, r0 + ir, n0 + in, v);
+        const int64_t row = r0 + ir, col = n0 + in;
+        const int valid = valid4(col, a.cols);
+        if (row >= it.hi || !valid) continue;
+        if constexpr (sizeof(T) == 4) {
+            if (it.group < a.groups && !finite(v[0] + v[1] + v[2] + v[3]))
+                for (int k = 0; k < valid; ++k)
+                    if (!finite(v[k])) v[k] = product_again<T, LB>(a, b, row, col + k);
+        }
+        store4<T>((T*)a.out + row * a.cols + col, v + bias4<T>(a, it, col), valid);
     }
 }
 
@@ -700,7 +758,7 @@ __global__ __launch_bounds__(THREADS, 2) void grouped_wgrad_kernel(GroupedArgs a
     __shared__ __attribute__((aligned(16))) typename X::E s0[X::stage];
     __shared__ __attribute__((aligned(16))) typename X::E s1[DIRECT ? X::stage : 8];
     const int tiles = a.row_tiles * a.col_tiles;
-    const int64_t id = blockIdx.x / tiles;
+    const int id = blockIdx.x / tiles;
     const int tile = blockIdx.x % tiles;
     const Item it = find_item<THREADS>(a, id, a.chunk, 1, false);
     if (it.group < 0) return;
@@ -732,24 +790,38 @@ __global__ __launch_bounds__(THREADS, 2) void grouped_wgrad_kernel(GroupedArgs a
     });
     const int64_t size = (int64_t)a.out_rows * a.cols;
     const int64_t slab = size + (BIAS ? a.cols : 0);
-    float* part = it.parts > 1 ? a.slabs + id * slab : nullptr;
-    X::each(acc, [&](int ir, int in, f32x4& v) {
-        const int64_t row = r0 + ir, col = n0 + in;
-        if (row >= a.out_rows || col >= a.cols) return;
-        const int valid = a.cols - col < 4 ? (int)(a.cols - col) : 4;
-        if constexpr (sizeof(T) == 4) {
+    float* part = it.parts > 1 ? a.slabs + (int64_t)id * slab : nullptr;
+    auto again = [&](int64_t row, int64_t col) {
+        float v = 0.0f;
+        for (int64_t c = c_lo; c < c_hi; ++c)
+            v = __builtin_fmaf((float)r[c * a.r_pitch + row], (float)b[c * a.b_pitch + col], v);
+        return v;
+    };
+    if constexpr (sizeof(T) == 4) {
+        if (any_lost(acc)) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                if (finite(v[k]) || k >= valid) continue;
-                float s = 0.0f;
-                for (int64_t c = c_lo; c < c_hi; ++c)
-                    s = __builtin_fmaf(r[c * a.r_pitch + row], b[c * a.b_pitch + col + k], s);
-                v[k] = s;
-            }
+            for (int i = 0; i < X::NR; ++i)
+#pragma unroll
+                for (int j = 0; j < X::NN; ++j)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (r0 + X::row(i) < a.out_rows && n0 + X::col(j) + k < a.cols && !finite(acc[i][j][k]))
+                            acc[i][j][k] = again(r0 + X::row(i), n0 + X::col(j) + k);
         }
-        if (part) store4<float>(part + row * a.cols + col, v, valid);
-        else store4<T>((T*)a.out + (int64_t)it.group * size + row * a.cols + col, v, valid);
-    });
+    }
+#pragma unroll
+    for (int i = 0; i < X::NR; ++i) {
+        const int64_t row = r0 + X::row(i);
+        if (row >= a.out_rows) continue;
+#pragma unroll
+        for (int j = 0; j < X::NN; ++j) {
+            const int64_t col = n0 + X::col(j);
+            const int valid = valid4(col, a.cols);
+            if (!valid) continue;
+            if (part) store4<float>(part + row * a.cols + col, acc[i][j], valid);
+            else store4<T>((T*)a.out + (int64_t)it.group * size + row * a.cols + col, acc[i][j], valid);
+        }
+    }
     if constexpr (!BIAS) return;
     if (!want_b) return;
     // the threads whose pieces have the same columns, in order
@@ -846,10 +918,12 @@ constexpr int64_t kBigTiles = 512;
 constexpr int kFewRows = 32;  // rows a group on average, up to which grouped_few_rows_kernel runs
 
 // Rows of a chunk of the weight gradient: whole groups where the weight alone has tiles enough to
-// fill the chip, else as many rows as leave about two workgroups per CU.
-int64_t wgrad_chunk(int64_t rows, int64_t groups, int64_t k, int64_t n) {
+// fill the chip, else as many rows as leave two workgroups per CU (more chunks are more slabs to write and
+// add: 208k rows, 237 groups, 128 x 128 bf16 41 us, 48 with four). With many tiles of fp32, whose workgroups
+// run longer, uneven groups want four (20k rows, 8 groups, 1024 x 1024: 272 us, 342 with two).
+int64_t wgrad_chunk(int64_t rows, int64_t groups, int64_t k, int64_t n, int eb) {
     const int64_t tiles = ((k + kTile - 1) / kTile) * ((n + kTile - 1) / kTile);
-    const int64_t want = 512 / tiles;  // chunks over all groups
+    const int64_t want = (eb == 4 && tiles > 4 ? 1024 : 512) / tiles;  // chunks over all groups
     if (want <= groups || rows == 0) return std::max<int64_t>(rows, 1);
     const int64_t c = (rows + want - 1) / want;
     return std::max<int64_t>(256, (c + 63) / 64 * 64);
@@ -935,12 +1009,14 @@ int32_t launch_wgrad(GroupedArgs a, hipStream_t strm) {
     a.col_tiles = (a.cols + TILE - 1) / TILE;
     const int64_t blocks = a.items * a.row_tiles * a.col_tiles;
     if (blocks > INT32_MAX) return unsupported("grouped linear: more than 2^31 tiles");
-    if (a.dbias)
-        hipLaunchKernelGGL((grouped_wgrad_kernel<T, TILE, TILE, THREADS, DIRECT, true>), dim3((unsigned)blocks),
-                           dim3(THREADS), 0, strm, a);
-    else
-        hipLaunchKernelGGL((grouped_wgrad_kernel<T, TILE, TILE, THREADS, DIRECT, false>), dim3((unsigned)blocks),
-                           dim3(THREADS), 0, strm, a);
+    const dim3 grid((unsigned)blocks), block(THREADS);
+    if constexpr (TILE == kTile) {
+        if (a.dbias) {
+            hipLaunchKernelGGL((grouped_wgrad_kernel<T, TILE, TILE, THREADS, DIRECT, true>), grid, block, 0, strm, a);
+            return MPGNN_OK;
+        }
+    }
+    hipLaunchKernelGGL((grouped_wgrad_kernel<T, TILE, TILE, THREADS, DIRECT, false>), grid, block, 0, strm, a);
     return MPGNN_OK;
 }
 
@@ -951,7 +1027,8 @@ int32_t wgrad_product(GroupedArgs a, hipStream_t strm) {
     if constexpr (sizeof(T) == 2) {
         const bool direct = direct_ok<T>(a);
         const int64_t tiles = (int64_t)((a.out_rows + 255) / 256) * ((a.cols + 255) / 256) * a.groups;
-        if (direct && big_cols(a.out_rows) && big_cols(a.cols) && a.rows >= 256 * (int64_t)a.groups && tiles >= kBigTiles)
+        // (with column sums the large tile has no registers left)
+        if (direct && !a.dbias && big_cols(a.out_rows) && big_cols(a.cols) && a.rows >= 256 * (int64_t)a.groups && tiles >= kBigTiles)
             st = launch_wgrad<T, 256, 512, true>(a, strm);
         else if (direct) st = launch_wgrad<T, kTile, 256, true>(a, strm);
         else st = launch_wgrad<T, kTile, 256, false>(a, strm);
@@ -1007,8 +1084,12 @@ extern "C" int32_t mpgnn_grouped_linear_wgrad_workspace_bytes(int64_t rows, int6
     int32_t st = check_grouped(rows, groups, k, n, MPGNN_F32, 64);
     if (st != MPGNN_OK) return st;
     if (!bytes) return arg_error("mpgnn_grouped_linear_wgrad_workspace_bytes: bytes is null");
-    const int64_t chunk = wgrad_chunk(rows, groups, k, n);
-    *bytes = rows > chunk ? wgrad_items(rows, groups, chunk) * (k * n + n) * (int64_t)sizeof(float) : 0;
+    *bytes = 0;
+    for (int eb : {2, 4}) {
+        const int64_t chunk = wgrad_chunk(rows, groups, k, n, eb);
+        if (rows > chunk)
+            *bytes = std::max(*bytes, wgrad_items(rows, groups, chunk) * (k * n + n) * (int64_t)sizeof(float));
+    }
     return MPGNN_OK;
 }
 
@@ -1021,7 +1102,7 @@ extern "C" int32_t mpgnn_grouped_linear_wgrad(const void* x, int64_t x_pitch, co
     if (st != MPGNN_OK) return st;
     if (!dweight || !group_ptr || (rows > 0 && (!x || !dy)) || (rows > 1 && (x_pitch < k || dy_pitch < n)))
         return arg_error("mpgnn_grouped_linear_wgrad: a null pointer, or a row pitch below the width");
-    const int64_t chunk = wgrad_chunk(rows, groups, k, n);
+    const int64_t chunk = wgrad_chunk(rows, groups, k, n, dtype_bytes(dtype));
     if (rows > chunk && !workspace) return arg_error("mpgnn_grouped_linear_wgrad: no workspace");
     if (chunk > INT32_MAX) return unsupported("mpgnn_grouped_linear_wgrad: over 2^31 rows");
     GroupedArgs a{};

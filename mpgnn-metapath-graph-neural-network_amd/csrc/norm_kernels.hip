@@ -66,6 +66,50 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float* lds, int& turn) {
     }
 }
 
+// The mean of a row and its summed squared differences from the mean, from those of each thread's n values:
+// two equal parts join to the mean of their means and the sum of their squares plus what the means differ by.
+// One exchange where a mean first and differences from it after take two.
+template <int TPR>
+__device__ __forceinline__ void join_stats(float& mean, float& m2, float n, float* lds, int& turn) {
+    constexpr int LANES = TPR < 64 ? TPR : 64;
+#pragma unroll
+    for (int d = 1; d < LANES; d <<= 1) {
+        const float om = __shfl_xor(mean, d, 64), os = __shfl_xor(m2, d, 64);
+        const float dm = om - mean;
+        mean = 0.5f * (mean + om);
+        m2 = __builtin_fmaf(dm * dm, 0.5f * n, m2 + os);
+        n *= 2.0f;
+    }
+    if constexpr (TPR > 64) {
+        constexpr int W = TPR / 64;
+        float* buf = lds + turn * (W * 2);
+        turn ^= 1;
+        if (threadIdx.x % 64 == 0) {
+            buf[threadIdx.x / 64 * 2] = mean;
+            buf[threadIdx.x / 64 * 2 + 1] = m2;
+        }
+        __syncthreads();
+        float ms[W], qs[W];
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            ms[w] = buf[w * 2];
+            qs[w] = buf[w * 2 + 1];
+        }
+#pragma unroll
+        for (int d = 1; d < W; d <<= 1) {
+#pragma unroll
+            for (int w = 0; w < W; w += 2 * d) {
+                const float dm = ms[w + d] - ms[w];
+                ms[w] = 0.5f * (ms[w] + ms[w + d]);
+                qs[w] = __builtin_fmaf(dm * dm, 0.5f * n, qs[w] + qs[w + d]);
+            }
+            n *= 2.0f;
+        }
+        mean = ms[0];
+        m2 = qs[0];
+    }
+}
+
 template <int TPR>
 struct RowShape {
     static constexpr int threads = TPR > 256 ? TPR : 256;
@@ -117,6 +161,7 @@ __global__ __launch_bounds__(RowShape<TPR>::threads) void layer_norm_fwd_kernel(
             b[i][j] = a.b && c < F ? param_at<T>(a.b, a.w_f32, c) : 0.0f;
         }
     const float width = (float)F;
+    const bool full = F == TPR * NV * V;
     int turn = 0;
     const int64_t step = (int64_t)gridDim.x * S::rows;
     Row<T, V, TPR, NV> next;
@@ -132,19 +177,33 @@ __global__ __launch_bounds__(RowShape<TPR>::threads) void layer_norm_fwd_kernel(
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int j = 0; j < V; ++j) s[0] += v[i][j];
-        row_sum<TPR, 1>(s, lds, turn);
-        const float mean = s[0] / width;
-        float q[1] = {0.0f};
+        float mean, q[1] = {0.0f};
+        if (full) {  // every thread has as many values
+            const float own = s[0] * (1.0f / (NV * V));
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const bool in = (i * TPR + t) * V < F;
+            for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                v[i][j] -= mean;
-                if (in) q[0] = __builtin_fmaf(v[i][j], v[i][j], q[0]);
+                for (int j = 0; j < V; ++j) q[0] = __builtin_fmaf(v[i][j] - own, v[i][j] - own, q[0]);
+            mean = own;
+            join_stats<TPR>(mean, q[0], (float)(NV * V), lds, turn);
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int j = 0; j < V; ++j) v[i][j] -= mean;
+        } else {
+            row_sum<TPR, 1>(s, lds, turn);
+            mean = s[0] / width;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const bool in = (i * TPR + t) * V < F;
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    v[i][j] -= mean;
+                    if (in) q[0] = __builtin_fmaf(v[i][j], v[i][j], q[0]);
+                }
             }
+            row_sum<TPR, 1>(q, lds, turn);
         }
-        row_sum<TPR, 1>(q, lds, turn);
         const float rstd = 1.0f / sqrtf(q[0] / width + a.eps);
         if (!live) continue;
         T* y = (T*)a.out + r * F;
@@ -416,7 +475,7 @@ bool vec_ok(const NormArgs& a, int eb) {
 
 template <typename T>
 int32_t norm_fwd(const NormArgs& a, hipStream_t strm) {
-    constexpr int max_blocks = 256 * 16;
+    constexpr int max_blocks = 256 * 8;
     const bool done = vec_ok(a, sizeof(T)) ? launch_by_width<T, 16 / sizeof(T)>(a, false, max_blocks, strm)
                                            : launch_by_width<T, 1>(a, false, max_blocks, strm);
     if (!done)

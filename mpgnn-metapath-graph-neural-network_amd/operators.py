@@ -16,7 +16,7 @@ from __future__ import annotations
 
 import ctypes
 import math
-import struct
+from array import array
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -41,23 +41,39 @@ def _require(t: torch.Tensor, name: str) -> int:
     return code
 
 
-class _on:
-    """The tensor's device made current for the call (a launch goes to the current device)."""
-    __slots__ = ("device", "guard")
+def _call(device: torch.device, entry, *args) -> None:
+    """A C entry point on torch's current stream of ``device``, made the current device for the call (a
+    launch goes to the current device)."""
+    if device.index == torch.cuda.current_device():
+        st = entry(*args, _stream_of(device))
+    else:
+        with torch.cuda.device(device):
+            st = entry(*args, _stream_of(device))
+    if st:
+        check(st, entry.__name__)
 
-    def __init__(self, device):
-        self.device = device
-        self.guard = None
 
-    def __enter__(self):
-        if self.device.index != torch.cuda.current_device():
-            self.guard = torch.cuda.device(self.device)
-            self.guard.__enter__()
-        return _stream_of(self.device)
+_WS_BYTES: dict = {}  # (entry, sizes) -> bytes: they depend on the sizes only, asked once for each
 
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+
+def _workspace_bytes(entry, *sizes) -> int:
+    n = _WS_BYTES.get((entry.__name__, sizes))
+    if n is None:
+        out = ctypes.c_int64()
+        check(entry(*sizes, ctypes.byref(out)), entry.__name__)
+        if len(_WS_BYTES) >= 4096:  # ragged batches: every step may bring new sizes
+            _WS_BYTES.clear()
+        n = _WS_BYTES[(entry.__name__, sizes)] = out.value
+    return n
+
+
+def _once(backward):
+    """``once_differentiable`` where a graph of the backward is wanted; it costs a few us a call otherwise."""
+    guarded = once_differentiable(backward)
+
+    def run(ctx, dy):
+        return guarded(ctx, dy) if torch.is_grad_enabled() else backward(ctx, dy)
+    return run
 
 
 # ---------------------------------------------------------------------------------------
@@ -83,50 +99,42 @@ def _norm_forward(x, weight, bias, eps, code, wcode, keep):
     if keep:
         mean = stats.data_ptr()
         rstd = mean + 4 * rows
-    with _on(x.device) as stream:
-        st = lib.mpgnn_layer_norm_fwd(xr.data_ptr(), rows, x.shape[-1], pitch, code, _ptr(weight), _ptr(bias), wcode,
-                                      eps, y.data_ptr(), mean, rstd, stream)
-    if st:
-        check(st, "mpgnn_layer_norm_fwd")
+    _call(x.device, lib.mpgnn_layer_norm_fwd, xr.data_ptr(), rows, x.shape[-1], pitch, code, _ptr(weight), _ptr(bias),
+          wcode, eps, y.data_ptr(), mean, rstd)
     return y, xr, stats
 
 
 class _LayerNormFn(torch.autograd.Function):
+    # what the backward needs of sizes is worked out in the forward: autograd runs backwards of GPU tensors on
+    # a thread of its own, where Python is about three times as slow
     @staticmethod
     def forward(ctx, x, weight, bias, eps, code, wcode):
         y, xr, stats = _norm_forward(x, weight, bias, eps, code, wcode, True)
-        ctx.codes = code, wcode
-        ctx.save_for_backward(xr, weight, stats)
+        width = x.shape[-1]
+        rows = stats.shape[1]
+        params = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+        nbytes = max(16, _workspace_bytes(lib.mpgnn_layer_norm_bwd_workspace_bytes, rows, width)) if params else 0
+        ctx.stats = stats  # neither an input nor an output
+        ctx.meta = (rows, width, width if xr.is_contiguous() else xr.stride(0), code, wcode, nbytes, stats.data_ptr(),
+                    x.dtype if wcode == code else torch.float32)
+        ctx.save_for_backward(xr, weight)
         return y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
-        x, weight, stats = ctx.saved_tensors
-        code, wcode = ctx.codes
+        x, weight = ctx.saved_tensors
+        rows, width, pitch, code, wcode, nbytes, mean, pdt = ctx.meta
         nx, nw, nb = ctx.needs_input_grad[:3]
-        width = x.shape[-1]
-        rows = x.numel() // width
-        pitch = width if x.is_contiguous() else x.stride(0)
+        device = x.device
         dyr, _, dy_pitch = _rows_view(dy)
-        pdt = x.dtype if wcode == code else torch.float32
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if nx else None
-        dw = torch.empty(width, dtype=pdt, device=x.device) if nw else None
-        db = torch.empty(width, dtype=pdt, device=x.device) if nb else None
-        ws = None
-        if nw or nb:
-            nbytes = ctypes.c_int64()
-            check(lib.mpgnn_layer_norm_bwd_workspace_bytes(rows, width, ctypes.byref(nbytes)),
-                  "mpgnn_layer_norm_bwd_workspace_bytes")
-            # a buffer of its own per call: a captured backward keeps it in its graph's pool
-            ws = torch.empty(max(nbytes.value, 16), dtype=torch.uint8, device=x.device)
-        mean = stats.data_ptr()
-        with _on(x.device) as stream:
-            st = lib.mpgnn_layer_norm_bwd(dyr.data_ptr(), dy_pitch, x.data_ptr(), pitch, rows, width, code,
-                                          _ptr(weight), wcode, mean, mean + 4 * rows, _ptr(dx), _ptr(dw), _ptr(db),
-                                          _ptr(ws), stream)
-        if st:
-            check(st, "mpgnn_layer_norm_bwd")
+        dx = torch.empty_like(x, memory_format=torch.contiguous_format) if nx else None
+        dw = torch.empty(width, dtype=pdt, device=device) if nw else None
+        db = torch.empty(width, dtype=pdt, device=device) if nb else None
+        # a buffer of its own per call: a captured backward keeps it in its graph's pool
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+        _call(device, lib.mpgnn_layer_norm_bwd, dyr.data_ptr(), dy_pitch, x.data_ptr(), pitch, rows, width, code,
+              _ptr(weight), wcode, mean, mean + 4 * rows, _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws))
         return dx, dw, db, None, None, None
 
 
@@ -170,52 +178,44 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor = None, bias: torch.Tensor 
 def _grouped_forward(x, pitch, weight, bias, ptr, bits, code):
     groups, k, n = weight.shape
     y = torch.empty((x.shape[0], n), dtype=x.dtype, device=x.device)
-    with _on(x.device) as stream:
-        st = lib.mpgnn_grouped_linear_fwd(x.data_ptr(), x.shape[0], pitch, code, weight.data_ptr(), groups, k, n,
-                                          _ptr(bias), ptr.data_ptr(), bits, y.data_ptr(), stream)
-    if st:
-        check(st, "mpgnn_grouped_linear_fwd")
+    _call(x.device, lib.mpgnn_grouped_linear_fwd, x.data_ptr(), x.shape[0], pitch, code, weight.data_ptr(), groups, k, n,
+          _ptr(bias), ptr.data_ptr(), bits, y.data_ptr())
     return y
 
 
 class _GroupedLinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, ptr, bits, code):
-        xr, _, pitch = _rows_view(x)
+        xr, rows, pitch = _rows_view(x)
         wc = weight if weight.is_contiguous() else weight.contiguous()
         bc = bias if bias is None or bias.is_contiguous() else bias.contiguous()
-        ctx.meta = pitch, bits, code
+        sizes = tuple(wc.shape)
+        params = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+        nbytes = _workspace_bytes(lib.mpgnn_grouped_linear_wgrad_workspace_bytes, rows, *sizes) if params else 0
+        ctx.meta = rows, pitch, bits, code, sizes, nbytes
         ctx.save_for_backward(xr, wc, ptr)
         return _grouped_forward(xr, pitch, wc, bc, ptr, bits, code)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
         x, weight, ptr = ctx.saved_tensors
-        pitch, bits, code = ctx.meta
+        rows, pitch, bits, code, sizes, nbytes = ctx.meta
         nx, nw, nb = ctx.needs_input_grad[:3]
-        groups, k, n = weight.shape
-        rows = x.shape[0]
+        device, p = x.device, ptr.data_ptr()
         dyr, _, dy_pitch = _rows_view(dy)
-        dx = torch.empty((rows, k), dtype=x.dtype, device=x.device) if nx else None
-        dw = torch.empty((groups, k, n), dtype=x.dtype, device=x.device) if nw or nb else None
-        db = torch.empty((groups, n), dtype=x.dtype, device=x.device) if nb else None
-        with _on(x.device) as stream:
-            if nx:
-                st = lib.mpgnn_grouped_linear_dgrad(dyr.data_ptr(), rows, dy_pitch, code, weight.data_ptr(), groups, k,
-                                                    n, ptr.data_ptr(), bits, dx.data_ptr(), stream)
-                if st:
-                    check(st, "mpgnn_grouped_linear_dgrad")
-            if nw or nb:
-                nbytes = ctypes.c_int64()
-                check(lib.mpgnn_grouped_linear_wgrad_workspace_bytes(rows, groups, k, n, ctypes.byref(nbytes)),
-                      "mpgnn_grouped_linear_wgrad_workspace_bytes")
-                ws = torch.empty(nbytes.value, dtype=torch.uint8, device=x.device) if nbytes.value else None
-                st = lib.mpgnn_grouped_linear_wgrad(x.data_ptr(), pitch, dyr.data_ptr(), dy_pitch, rows, code, groups,
-                                                    k, n, ptr.data_ptr(), bits, dw.data_ptr(), _ptr(db), _ptr(ws),
-                                                    stream)
-                if st:
-                    check(st, "mpgnn_grouped_linear_wgrad")
+        dx = dw = db = None
+        if nx:
+            dx = torch.empty_like(x, memory_format=torch.contiguous_format)
+            _call(device, lib.mpgnn_grouped_linear_dgrad, dyr.data_ptr(), rows, dy_pitch, code, weight.data_ptr(), *sizes,
+                  p, bits, dx.data_ptr())
+        if nw or nb:
+            dw = torch.empty_like(weight)
+            if nb:
+                db = torch.empty((sizes[0], sizes[2]), dtype=x.dtype, device=device)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+            _call(device, lib.mpgnn_grouped_linear_wgrad, x.data_ptr(), pitch, dyr.data_ptr(), dy_pitch, rows, code,
+                  *sizes, p, bits, dw.data_ptr(), _ptr(db), _ptr(ws))
         return dx, dw if nw else None, db, None, None, None
 
 
@@ -265,11 +265,36 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, group_ptr: torch.Tenso
 # ---------------------------------------------------------------------------------------
 # global norm and clipping
 # ---------------------------------------------------------------------------------------
-_CLIP_RECORD = struct.Struct("=QQqii")  # mpgnn_clip_tensor
+def _describe(tensors, what) -> tuple[list, list]:
+    """(mpgnn_dtype codes, element counts) of tensors that lie dense on one GPU; a column of the list at
+    a time, as with hundreds of tensors a step these checks are the calls' host time."""
+    codes = [_DTYPE.get(d) for d in [t.dtype for t in tensors]]
+    if None in codes or not tensors[0].is_cuda or len({t.get_device() for t in tensors}) != 1:
+        device = tensors[0].device
+        for t in tensors:
+            _require(t, what)
+            if t.device != device:
+                raise RuntimeError(f"{what} are on several devices: {device} and {t.device}")
+    return codes, [t.numel() for t in tensors]
 
 
-def _clip(grads, outs, max_norm, norm_type) -> torch.Tensor:
-    """The norm of ``grads`` (one device, contiguous); ``outs``: where the scaled tensors go, or None."""
+def _contiguous(tensors, what) -> list:
+    """Indices of the tensors that are not contiguous."""
+    try:
+        flags = [t.is_contiguous() for t in tensors]
+    except RuntimeError as exc:  # a sparse layout
+        raise TypeError(f"mpgnn_amd: {what} must be dense") from exc
+    if False not in flags:
+        return []
+    strided = [k for k, c in enumerate(flags) if not c]
+    for k in strided:
+        if tensors[k].layout is not torch.strided:
+            raise TypeError(f"mpgnn_amd: {what} must be dense, got {tensors[k].layout}")
+    return strided
+
+
+def _clip(grads, codes, numels, outs, max_norm, norm_type) -> torch.Tensor:
+    """The norm of ``grads`` (checked and contiguous); ``outs``: where the scaled tensors go, or None."""
     if norm_type == 2.0:
         kind = NORM_2
     elif norm_type == math.inf:
@@ -278,38 +303,28 @@ def _clip(grads, outs, max_norm, norm_type) -> torch.Tensor:
         raise ValueError(f"norm_type must be 2 or inf, got {norm_type!r}")
     n = len(grads)
     device = grads[0].device
-    # the records packed at once: hundreds of tensors a step make this loop the call's host time
-    pack = _CLIP_RECORD.pack
-    if outs is None:
-        table = b"".join([pack(g.data_ptr(), 0, g.numel(), _DTYPE[g.dtype], 0) for g in grads])
-    elif outs is grads:
-        table = b"".join([pack(p, p, g.numel(), _DTYPE[g.dtype], 0) for g in grads for p in (g.data_ptr(),)])
-    else:
-        table = b"".join([pack(g.data_ptr(), o.data_ptr(), g.numel(), _DTYPE[g.dtype], 0)
-                          for g, o in zip(grads, outs)])
-    nbytes = ctypes.c_int64()
-    st = lib.mpgnn_clip_workspace_bytes(n, ctypes.byref(nbytes))
-    if st:
-        check(st, "mpgnn_clip_workspace_bytes")
-    ws = torch.empty(nbytes.value, dtype=torch.uint8, device=device)
+    # mpgnn_clip_tensor records: four 64-bit words (grad, out, numel, dtype)
+    words = array("q", bytes(32 * n))
+    words[0::4] = array("q", [g.data_ptr() for g in grads])
+    if outs is grads:
+        words[1::4] = words[0::4]
+    elif outs is not None:
+        words[1::4] = array("q", [o.data_ptr() for o in outs])
+    if outs is not None and len(set(words[1::4])) != n:
+        # each tensor with elements at an address of its own: scaled in place twice, one would be scaled by
+        # the factor's square
+        used = [p for p, m in zip(words[1::4], numels) if m]
+        if len(set(used)) != len(used):
+            raise ValueError("one tensor is to be scaled twice")
+    words[2::4] = array("q", numels)
+    words[3::4] = array("q", codes)
+    ws = torch.empty(_workspace_bytes(lib.mpgnn_clip_workspace_bytes, n), dtype=torch.uint8, device=device)
     norm = torch.empty((), dtype=torch.float32, device=device)
-    with _on(device) as stream:
-        st = lib.mpgnn_clip_by_global_norm(table, n, kind, max_norm, norm.data_ptr(), ws.data_ptr(), stream)
-    if st:
-        check(st, "mpgnn_clip_by_global_norm")
+    _call(device, lib.mpgnn_clip_by_global_norm, words.buffer_info()[0], n, kind, max_norm, norm.data_ptr(),
+          ws.data_ptr())
     if outs is not None:
         increment_version(outs)  # written behind autograd's back, as any in-place operator counts
     return norm
-
-
-def _check_list(tensors, what):
-    device = tensors[0].device
-    for t in tensors:
-        if not (t.is_cuda and t.dtype in _DTYPE and t.layout is torch.strided and t.device == device):
-            if t.layout is not torch.strided:
-                raise TypeError(f"mpgnn_amd: {what} must be dense, got {t.layout}")
-            _require(t, what)
-            raise RuntimeError(f"{what} are on several devices: {device} and {t.device}")
 
 
 def _check_max_norm(max_norm) -> float:
@@ -319,20 +334,10 @@ def _check_max_norm(max_norm) -> float:
     return max_norm
 
 
-def _distinct(tensors, what):
-    """Each tensor with elements starts at an address of its own: scaled in place twice, one would
-    be scaled by the factor's square."""
-    ptrs = [t.data_ptr() for t in tensors]
-    if len(set(ptrs)) != len(ptrs):  # empty tensors may share one
-        ptrs = [t.data_ptr() for t in tensors if t.numel()]
-        if len(set(ptrs)) != len(ptrs):
-            raise ValueError(f"{what} holds one tensor twice")
-
-
 def clip_by_global_norm(tensors, max_norm: float, norm_type: float = 2.0, out=None):
     """``(norm, clipped)``: the global norm over ``tensors`` (the 2-norm of all elements, or the largest
     magnitude with ``norm_type=inf``) as an fp32 scalar tensor, and ``t * min(1, max_norm / (norm + 1e-6))``
-    of each, in new tensors or in those of ``out`` (same shapes, types and device, contiguous; ``out`` may
+    of each, in new tensors or in those of ``out`` (same sizes, types and device, contiguous; ``out`` may
     be ``tensors`` itself, otherwise the two must not overlap). Not differentiable; no host synchronisation.
 
     The factor is computed and applied in fp32 and each product rounded once to its tensor's type. An
@@ -341,19 +346,20 @@ def clip_by_global_norm(tensors, max_norm: float, norm_type: float = 2.0, out=No
     tensors = list(tensors)
     if not tensors:
         raise ValueError("clip_by_global_norm needs at least one tensor")
-    _check_list(tensors, "tensors")
+    codes, numels = _describe(tensors, "tensors")
+    strided = _contiguous(tensors, "tensors")
     if out is None:
         outs = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in tensors]
     else:
         outs = list(out)
         if len(outs) != len(tensors):
             raise ValueError(f"out has {len(outs)} tensors for {len(tensors)}")
-        for o, t in zip(outs, tensors):
-            if not (o.dtype == t.dtype and o.shape == t.shape and o.device == t.device and o.is_contiguous()):
-                raise ValueError("out must hold contiguous tensors of the inputs' shapes, types and device")
-        _distinct(outs, "out")
-    grads = [t if t.is_contiguous() else t.detach().contiguous() for t in tensors]
-    return _clip(grads, outs, max_norm, norm_type), outs
+        if _describe(outs, "out") != (codes, numels) or outs[0].device != tensors[0].device or \
+                _contiguous(outs, "out"):
+            raise ValueError("out must hold contiguous tensors of the inputs' sizes, types and device")
+    for k in strided:
+        tensors[k] = tensors[k].detach().contiguous()
+    return _clip(tensors, codes, numels, outs, max_norm, norm_type), outs
 
 
 def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False,
@@ -371,12 +377,13 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_i
     grads = [g for g in (p.grad for p in parameters) if g is not None]
     if not grads:
         return torch.tensor(0.0)
-    _check_list(grads, "gradients")
-    _distinct(grads, "the parameters' gradients")
+    codes, numels = _describe(grads, "gradients")
+    strided = _contiguous(grads, "gradients")
     flat = grads
-    strided = [k for k, g in enumerate(grads) if not g.is_contiguous()]
     if strided:
         flat = list(grads)
+        if len({id(g) for g in grads}) != len(grads):
+            raise ValueError("one tensor is to be scaled twice")
         for k in strided:
             g = grads[k]
             if any(st == 0 and n > 1 for n, st in zip(g.shape, g.stride())):
@@ -384,12 +391,12 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_i
                                  "in place")
             flat[k] = g.detach().contiguous()
     if error_if_nonfinite:
-        norm = _clip(flat, None, max_norm, norm_type)
+        norm = _clip(flat, codes, numels, None, max_norm, norm_type)
         if not math.isfinite(float(norm)):
             raise RuntimeError(f"The total norm of order {norm_type} for gradients from `parameters` is non-finite, so "
                                "it cannot be clipped. To disable this error and scale the gradients by the non-finite "
                                "norm anyway, set `error_if_nonfinite=False`")
-    norm = _clip(flat, flat, max_norm, norm_type)
+    norm = _clip(flat, codes, numels, flat, max_norm, norm_type)
     if strided:
         with torch.no_grad():
             for k in strided:
