@@ -17,6 +17,7 @@ import torch
 from . import data as _data
 from .metrics import class_weight_balanced, confusion_counts_rows, f1_from_counts, nll_loss_rows
 from .model import MPNetm
+from .operators import clip_grad_norm_
 # score function helpers of main.py:387-917 (both branches, GPU kernels): same names, plus the
 # batched first-round scoring of every relation (score_relations_batched)
 from .score import (clean_bags_for_relation_type, create_bags, create_edge_dictionary,  # noqa: F401
@@ -316,23 +317,26 @@ def take_rows(out: torch.Tensor, idx):
     return out[idx]
 
 
-def _train_step(model, optimizer, data):
-    """mpgnn_train's body with the loss left on the device (no host sync)."""
+def _train_step(model, optimizer, data, max_grad_norm=None):
+    """mpgnn_train's body with the loss left on the device (no host sync). ``max_grad_norm``: the
+    gradients clipped to that global norm before the step (``operators.clip_grad_norm_``)."""
     model.train()
     optimizer.zero_grad()
     out = model(data.x, data.edge_index, data.edge_type)
     weights = class_weight_balanced(data.train_y)
     loss = nll_loss_rows(out, data.train_idx, data.train_y)
     loss.backward()
+    if max_grad_norm is not None:
+        clip_grad_norm_(model.parameters(), max_grad_norm)
     optimizer.step()
     return loss.detach(), weights
 
 
-def mpgnn_train(model, optimizer, data):
+def mpgnn_train(model, optimizer, data, max_grad_norm=None):
     """main.py:1055-1082: full-batch forward, unweighted NLL on train_idx, backward, step.
     Returns (float loss, balanced class weights) like the reference (the weights are
-    computed there but not applied, main.py:1065)."""
-    loss, weights = _train_step(model, optimizer, data)
+    computed there but not applied, main.py:1065). ``max_grad_norm`` (an addition): see _train_step."""
+    loss, weights = _train_step(model, optimizer, data, max_grad_norm)
     return float(loss), weights
 
 
@@ -367,7 +371,8 @@ def mpgnn_test(model, data, class_weight):
     return loss_test, f1_test
 
 
-def _fit(data_mpgnn, input_dim, hidden_dim, num_rel, output_dim, ll_output_dim, metapaths, epochs):
+def _fit(data_mpgnn, input_dim, hidden_dim, num_rel, output_dim, ll_output_dim, metapaths, epochs,
+         max_grad_norm=None):
     model = MPNetm(input_dim, hidden_dim, num_rel, output_dim, ll_output_dim, len(metapaths), metapaths)
     model = model.to(data_mpgnn.x.device)
     optimizer = None if _graphs_enabled(data_mpgnn) else _adam(model)
@@ -381,7 +386,7 @@ def _fit(data_mpgnn, input_dim, hidden_dim, num_rel, output_dim, ll_output_dim, 
     # every epoch trains and scores the validation split on the device; only the last epoch's
     # score is read by the host (its best-score test only re-assigns the same model object)
     def epoch():
-        loss, _ = _train_step(model, optimizer, data_mpgnn)
+        loss, _ = _train_step(model, optimizer, data_mpgnn, max_grad_norm)
         return (loss,) + _val_counts(model, data_mpgnn)
 
     for _epoch, (_loss, _loss_val, vcounts) in _epochs(epoch, epochs, use_graph):
@@ -391,24 +396,25 @@ def _fit(data_mpgnn, input_dim, hidden_dim, num_rel, output_dim, ll_output_dim, 
 
 
 def mpgnn_parallel_multiple(data_mpgnn, input_dim, hidden_dim, num_rel, output_dim, ll_output_dim, metapaths,
-                            epochs: int = EPOCHS):
+                            epochs: int = EPOCHS, max_grad_norm=None):
     """main.py:1117-1136: train an MPNetm over ``metapaths`` for 999 epochs with Adam
-    (lr 0.01, wd 5e-4); returns the last epoch's validation macro F1."""
+    (lr 0.01, wd 5e-4); returns the last epoch's validation macro F1. ``max_grad_norm`` (an addition):
+    the gradients clipped to that global norm before each step."""
     _, best_model, class_weight, f1_valt_macro = _fit(data_mpgnn, input_dim, hidden_dim, num_rel, output_dim,
-                                                      ll_output_dim, metapaths, epochs)
+                                                      ll_output_dim, metapaths, epochs, max_grad_norm)
     mpgnn_test(best_model, data_mpgnn, class_weight)
     return f1_valt_macro
 
 
 def mpgnn_parallel_multiple_x(data_mpgnn, input_dim, hidden_dim, num_rel, output_dim, ll_output_dim, metapaths,
-                              testing, epochs: int = EPOCHS):
+                              testing, epochs: int = EPOCHS, max_grad_norm=None):
     """main.py:1138-1160: as ``mpgnn_parallel_multiple`` (a single metapath may be given as a
     flat list); prints the test line; returns the test macro F1 when ``testing`` else the last
     validation macro F1."""
     if isinstance(metapaths[0], int):
         metapaths = [metapaths]
     _, best_model, class_weight, f1_valt_macro = _fit(data_mpgnn, input_dim, hidden_dim, num_rel, output_dim,
-                                                      ll_output_dim, metapaths, epochs)
+                                                      ll_output_dim, metapaths, epochs, max_grad_norm)
     test_loss, f1_macro_test = mpgnn_test(best_model, data_mpgnn, class_weight)
     print("test loss %0.3f" % test_loss, "test macro %0.3f" % f1_macro_test)
     if testing == False:  # noqa: E712  (reference: 0 and False both select validation)

@@ -19,6 +19,7 @@ from .main import (_adam, _adam_graphable, _epochs, _graphs_enabled, _one_hot_co
                    get_edge_index_and_type_no_reverse, load_files, load_graph, take_rows)
 from .metrics import class_weight_balanced, class_weight_tensor, confusion_counts_rows, f1_from_counts, nll_loss_rows
 from .model import Net
+from .operators import clip_grad_norm_
 
 __all__ = ["Data", "get_node_features", "mpgnn_train", "mpgnn_validation", "mpgnn_test", "mpgnn_parallel_multiple", "EPOCHS"]
 
@@ -36,8 +37,9 @@ def _forward(model, data):
     return model(data.x, data.edge_index, data.edge_type, **kw)
 
 
-def _train_step(model, optimizer, data):
-    """The body of mpgnn_train with the loss left on the device (no host sync)."""
+def _train_step(model, optimizer, data, max_grad_norm=None):
+    """The body of mpgnn_train with the loss left on the device (no host sync). ``max_grad_norm``: the
+    gradients clipped to that global norm before the step (``operators.clip_grad_norm_``)."""
     model.train()
     optimizer.zero_grad()
     out = _forward(model, data)
@@ -46,14 +48,17 @@ def _train_step(model, optimizer, data):
     # F.nll_loss(out[train_idx], train_y, weight=weights_tensor): one launch each way on the GPU
     loss = nll_loss_rows(out, data.train_idx, data.train_y, weight=weights_tensor)
     loss.backward()
+    if max_grad_norm is not None:
+        clip_grad_norm_(model.parameters(), max_grad_norm)
     optimizer.step()
     return loss.detach(), weights
 
 
-def mpgnn_train(model, optimizer, data):
+def mpgnn_train(model, optimizer, data, max_grad_norm=None):
     """main_rgcn.py:369-393: forward, NLL on train_idx weighted by the balanced class weights
-    (main_rgcn.py:376-380), backward, step → (float loss, weights)."""
-    loss, weights = _train_step(model, optimizer, data)
+    (main_rgcn.py:376-380), backward, step → (float loss, weights). ``max_grad_norm`` (an addition): see
+    _train_step."""
+    loss, weights = _train_step(model, optimizer, data, max_grad_norm)
     return float(loss), weights
 
 
@@ -99,12 +104,14 @@ def mpgnn_test(model, data, class_weight):
 
 
 def mpgnn_parallel_multiple(data_mpgnn, input_dim, hidden_dim, num_rel, output_dim, ll_output_dim, metapath_length,
-                            epochs: int = EPOCHS, verbose: bool = True):
+                            epochs: int = EPOCHS, verbose: bool = True, *, layer_norm: bool = False,
+                            max_grad_norm=None):
     """main_rgcn.py:452-472: train ``Net`` (L = metapath_length) for 999 epochs with Adam
     (lr 0.01, wd 5e-4), running train / validation / test every epoch and printing every
     10th; returns the test macro F1 of ``best_model`` (the same object as the trained model,
-    as in the reference)."""
-    model = Net(input_dim, hidden_dim, num_rel, output_dim, ll_output_dim, metapath_length)
+    as in the reference). ``layer_norm`` and ``max_grad_norm`` (additions): Net's, and the gradients
+    clipped to that global norm before each step."""
+    model = Net(input_dim, hidden_dim, num_rel, output_dim, ll_output_dim, metapath_length, layer_norm=layer_norm)
     model = model.to(data_mpgnn.x.device)
     use_graph = _graphs_enabled(data_mpgnn)
     optimizer = _adam_graphable(model) if use_graph else _adam(model)
@@ -117,7 +124,7 @@ def mpgnn_parallel_multiple(data_mpgnn, input_dim, hidden_dim, num_rel, output_d
     # best-score test changes nothing and needs no host read.
     # (one HIP graph per epoch after three eager ones: main._epochs)
     def epoch_fn():
-        loss, _ = _train_step(model, optimizer, data_mpgnn)
+        loss, _ = _train_step(model, optimizer, data_mpgnn, max_grad_norm)
         return (loss,) + _val_counts(model, data_mpgnn) + _test_counts(model, data_mpgnn)
 
     for epoch, (loss, loss_val, vcounts, test_loss, tcounts) in _epochs(epoch_fn, epochs, use_graph):

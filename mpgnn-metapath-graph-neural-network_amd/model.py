@@ -21,7 +21,7 @@ import torch.nn.functional as F
 
 from .mp_rgcn_layer import CustomRGCNConv
 from .functional import GradStash
-from .nn import RGCNConv
+from .nn import LayerNorm, RGCNConv
 from .score import InputLayer, OutputLayer, Score  # noqa: F401  (model.py:26-125)
 
 __all__ = ["Net", "MPNetm", "linear", "InputLayer", "OutputLayer", "Score"]
@@ -327,14 +327,21 @@ def _hooked(*mods) -> bool:
 
 
 class Net(_FastTrainToggle, torch.nn.Module):
-    """RGCN baseline (model.py:132-149): conv1, then the SAME conv2 for layers 1..L-1."""
+    """RGCN baseline (model.py:132-149): conv1, then the SAME conv2 for layers 1..L-1.
 
-    def __init__(self, input_dim, hidden_dim, num_rel, output_dim, ll_output_dim, metapath_length):
+    ``layer_norm=True`` (an addition to the reference) normalises each layer's activations
+    (``nn.LayerNorm``: norm1 after conv1, norm2 after every use of conv2); the parameters and their
+    order are the reference's otherwise."""
+
+    def __init__(self, input_dim, hidden_dim, num_rel, output_dim, ll_output_dim, metapath_length, *,
+                 layer_norm: bool = False):
         super().__init__()
         self.metapath_length = metapath_length
         self.conv1 = RGCNConv(input_dim, hidden_dim, num_rel, flow="target_to_source")
         self.conv2 = RGCNConv(hidden_dim, output_dim, num_rel, flow="target_to_source")
         self.LinearLayer = torch.nn.Linear(output_dim, ll_output_dim)
+        self.norm1 = LayerNorm(hidden_dim) if layer_norm else None
+        self.norm2 = LayerNorm(output_dim) if layer_norm else None
 
     def forward(self, x, edge_index, edge_type, *, shard=None, group=None, shard_side="gathered"):
         last = self.metapath_length - 1
@@ -357,7 +364,10 @@ class Net(_FastTrainToggle, torch.nn.Module):
             # F.relu(conv(...)) of model.py:144,146, fused into the layer's combine kernel
             x = conv(x, edge_index, edge_type, shard=shard, group=group, activation="relu", shard_side=shard_side,
                      **kw)
-            if internal:
+            norm = self.norm1 if layer_index == 0 else self.norm2
+            if norm is not None:
+                x = norm(x)
+            elif internal:
                 x._mpgnn_relu_internal = True
         return head_log_softmax(self.LinearLayer, x)  # F.log_softmax(self.LinearLayer(x), dim=1)
 

@@ -635,6 +635,68 @@ def test_results_repeat_bitwise():
     assert all(torch.equal(a, b) for r in runs[1:] for a, b in zip(r, runs[0]))
 
 
+def _small_graph_data():
+    from mpgnn_amd import data, main
+    g = data.synthetic_graph(400, 4, 6, feat_dim=16, seed=3)
+    gen_ = gen(90)
+    idx = torch.randperm(400, generator=gen_)
+    y = torch.randint(0, 3, (400,), generator=gen_)
+    return main.Data(x=g.x, edge_index=g.edge_index, edge_type=g.edge_type, train_idx=idx[:200], train_y=y[idx[:200]],
+                     val_idx=idx[200:300], val_y=y[idx[200:300]], test_idx=idx[300:], test_y=y[idx[300:]]).to(DEV)
+
+
+def test_net_with_layer_norm_and_clipped_step():
+    """Net(layer_norm=True): its forward and gradients equal those of the same model with torch's own
+    LayerNorm modules in place; the training step then clips what it steps with."""
+    from mpgnn_amd import main_rgcn
+    data = _small_graph_data()
+    torch.manual_seed(5)
+    net = mpgnn_amd.Net(16, 32, 4, 32, 3, 3, layer_norm=True).to(DEV)
+    assert sorted(set(net.state_dict()) - set(mpgnn_amd.Net(16, 32, 4, 32, 3, 3).state_dict())) == \
+        ["norm1.bias", "norm1.weight", "norm2.bias", "norm2.weight"]
+    with torch.no_grad():
+        for p in (net.norm1.weight, net.norm2.weight):
+            p.add_(torch.linspace(-0.5, 0.5, 32, device=DEV))
+    ref = mpgnn_amd.Net(16, 32, 4, 32, 3, 3).to(DEV)
+    ref.norm1, ref.norm2 = torch.nn.LayerNorm(32).to(DEV), torch.nn.LayerNorm(32).to(DEV)
+    ref.load_state_dict(net.state_dict())
+    outs = []
+    for m in (net, ref):
+        out = m(data.x, data.edge_index, data.edge_type)
+        out[data.train_idx].gather(1, data.train_y[:, None]).sum().neg().backward()
+        outs.append(out)
+    # both sides' norms are fp32 with errors of about 2^-22; three layers and a log-softmax of them
+    assert float((outs[0] - outs[1]).detach().abs().max()) <= 1e-4
+    for (n, a), b in zip(net.named_parameters(), ref.parameters()):
+        assert a.grad is not None, n
+        assert float((a.grad - b.grad).norm()) <= 1e-4 * float(b.grad.norm()) + 1e-6, n
+    opt = torch.optim.SGD(net.parameters(), lr=0.0)
+    main_rgcn.mpgnn_train(net, opt, data, max_grad_norm=1e-3)
+    total = math.sqrt(sum(float(p.grad.double().square().sum()) for p in net.parameters()))
+    assert 0.99e-3 <= total <= 1.001e-3
+
+
+def test_loops_take_the_additions(monkeypatch):
+    """The training loops with layer_norm and max_grad_norm, their epochs captured in a graph or not: the
+    same scores. Left out, nothing changes."""
+    from mpgnn_amd import main, main_rgcn
+    data = _small_graph_data()
+    scores = {}
+    for graph in ("1", "0"):
+        monkeypatch.setenv("MPGNN_LOOP_GRAPH", graph)
+        torch.manual_seed(30)
+        scores[graph, "rgcn"] = main_rgcn.mpgnn_parallel_multiple(data, 16, 32, 4, 32, 3, 2, epochs=8, verbose=False,
+                                                                  layer_norm=True, max_grad_norm=0.5)
+        torch.manual_seed(30)
+        scores[graph, "mpgnn"] = main.mpgnn_parallel_multiple(data, 16, 32, 4, 32, 3, [[0, 1]], epochs=8,
+                                                              max_grad_norm=0.5)
+        torch.manual_seed(30)
+        scores[graph, "plain"] = main_rgcn.mpgnn_parallel_multiple(data, 16, 32, 4, 32, 3, 2, epochs=8, verbose=False)
+    assert scores["1", "rgcn"] == scores["0", "rgcn"]
+    assert scores["1", "plain"] == scores["0", "plain"]
+    assert all(0.0 <= float(v) <= 1.0 for v in scores.values())
+
+
 def test_gpu_refusals():
     x = torch.zeros(4, 8, device=DEV)
     with pytest.raises(TypeError):
