@@ -42,6 +42,8 @@ enum Layout { ALONG, ACROSS };  // c fastest, or the index fastest
 struct GroupedArgs {
     const void* r;      // rows operand
     const void* b;      // columns operand
+    const void* r_end;  // behind the last element of each
+    const void* b_end;
     void* out;
     const void* bias;   // forward: [G][cols] or null
     const void* ptr;    // [G + 1] int32 or int64
@@ -276,17 +278,39 @@ struct Tile {
             return read_across<typename Frag<E>::type>(p, p + 4 * IDX);  // c + 4 trades as c does
         }
     }
-    // the tile of `p` whose indices start at i0 (of i_n) and whose c at c0 (of c_n); outside: zero
+    // how many of the 8 elements at index i and c = k lie inside i_n and c_n
+    static __device__ __forceinline__ int inside(int64_t i, int64_t i_n, int64_t k, int64_t c_n) {
+        const int64_t left = L == ALONG ? (i < i_n ? c_n - k : 0) : (k < c_n ? i_n - i : 0);
+        return left >= 8 ? 8 : left > 0 ? (int)left : 0;
+    }
+    // The tile of `p` whose indices start at i0 (of i_n) and whose c at c0 (of c_n); outside: zero. All pieces are
+    // asked for before any is looked at: a piece that is cut is read whole and masked, unless that leads past
+    // `end`, the end of the tensor.
     static __device__ __forceinline__ void load(Raw<T> (&raw)[chunks], int tid, const T* p, int64_t pitch, int64_t i0,
-                                                int64_t i_n, int64_t c0, int64_t c_n) {
+                                                int64_t i_n, int64_t c0, int64_t c_n, const T* end) {
+        const T* at[chunks];
+        int valid[chunks];
 #pragma unroll
         for (int n = 0; n < chunks; ++n) {
             int idx, c;
             place(tid, n, idx, c);
-            const int64_t i = i0 + idx, k = c0 + c;
-            const int64_t left = L == ALONG ? (i < i_n ? c_n - k : 0) : (k < c_n ? i_n - i : 0);
-            const int valid = left >= 8 ? 8 : left > 0 ? (int)left : 0;
-            raw[n] = load8<T>(valid ? p + (L == ALONG ? i * pitch + k : k * pitch + i) : p, valid);
+            valid[n] = inside(i0 + idx, i_n, c0 + c, c_n);
+            at[n] = p + (L == ALONG ? (i0 + idx) * pitch + c0 + c : (c0 + c) * pitch + i0 + idx);
+            raw[n] = Raw<T>{};
+            if (valid[n] && at[n] + 8 <= end) __builtin_memcpy(&raw[n], at[n], sizeof(raw[n]));
+        }
+#pragma unroll
+        for (int n = 0; n < chunks; ++n) {
+            if (valid[n] == 8) continue;
+            T e[8];
+            __builtin_memcpy(e, &raw[n], sizeof(e));
+            const bool short_end = valid[n] && at[n] + 8 > end;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                if (k >= valid[n]) e[k] = (T)0.0f;
+                else if (short_end) e[k] = at[n][k];
+            }
+            __builtin_memcpy(&raw[n], e, sizeof(e));
         }
     }
     static __device__ __forceinline__ void store(E* lds, int tid, const Raw<T> (&raw)[chunks]) {
@@ -306,8 +330,7 @@ struct Tile {
             int idx, c;
             place(tid, n, idx, c);
             const int64_t i = i0 + idx, k = c0 + c;
-            const int64_t left = L == ALONG ? (i < i_n ? c_n - k : 0) : (k < c_n ? i_n - i : 0);
-            const int valid = left >= 8 ? 8 : left > 0 ? (int)left : 0;
+            const int valid = inside(i, i_n, k, c_n);
             store8<T>(lds + offset(idx, c), plane,
                       load8<T>(valid ? p + (L == ALONG ? i * pitch + k : k * pitch + i) : p, valid));
         }
@@ -354,37 +377,59 @@ struct Tile {
         const T* base;
         int64_t step;
 
+        int end, pitch_;
+
         __device__ __forceinline__ Direct(const T* p, int64_t pitch, int64_t i0, int64_t i_n, int64_t c0) {
             wave_at = __builtin_amdgcn_readfirstlane(threadIdx.x / 64) * 1024;
-            const int end = i_n - i0 < IDX ? (int)(i_n - i0) : IDX;  // at least 1; ACROSS: at least 8
+            end = i_n - i0 < IDX ? (int)(i_n - i0) : IDX;  // at least 1; ACROSS: at least 8
+            pitch_ = (int)pitch;
 #pragma unroll
-            for (int n = 0; n < chunks; ++n) {
-                const int slot = n * THREADS + threadIdx.x;  // 16-byte piece of the tile in LDS
-                if constexpr (L == ALONG) {
-                    const int idx = slot / (BK / 8);
-                    at[n] = (unsigned)((idx < end ? idx : end - 1) * (int)pitch + ((slot % (BK / 8)) ^ turn(idx)) * 8) * 2;
-                } else {
-                    const int c = slot / (IDX / 8), s = slot % (IDX / 8);
-                    const int idx = ((s / 2) ^ trade(c)) * 16 + s % 2 * 8;
-                    at[n] = (unsigned)(c * (int)pitch + (idx < end ? idx : end - 8)) * 2;
-                }
-            }
+            for (int n = 0; n < chunks; ++n) at[n] = reach(n, BK);
             base = L == ALONG ? p + i0 * pitch + c0 : p + c0 * pitch + i0;
             step = L == ALONG ? BK : BK * pitch;
         }
+        // bytes from the base to piece n of the wave's lanes, with c kept inside the first `left` (ALONG: at
+        // least 8 of them)
+        __device__ __forceinline__ unsigned reach(int n, int left) const {
+            const int slot = n * THREADS + threadIdx.x;  // 16-byte piece of the tile in LDS
+            if constexpr (L == ALONG) {
+                const int idx = slot / (BK / 8), c = ((slot % (BK / 8)) ^ turn(idx)) * 8;
+                return (unsigned)((idx < end ? idx : end - 1) * pitch_ + (c < left ? c : left - 8)) * 2;
+            } else {
+                const int c = slot / (IDX / 8), s = slot % (IDX / 8);
+                const int idx = ((s / 2) ^ trade(c)) * 16 + s % 2 * 8;
+                return (unsigned)((c < left ? c : left - 1) * pitch_ + (idx < end ? idx : end - 8)) * 2;
+            }
+        }
         // (Written out, as the compiler would wait for every load before it reads any stage. The wait states are the
         // ones that m0 needs before a load to LDS and that a scalar from a vector lane needs before a load.)
-        __device__ __forceinline__ void next(E* lds) {
+        template <typename F>
+        __device__ __forceinline__ void send(E* lds, F&& from) const {
             typedef __attribute__((address_space(3))) E* lptr;
             const unsigned to = __builtin_amdgcn_readfirstlane((unsigned)(unsigned long long)(lptr)lds + wave_at);
-            const int64_t from = scalar((int64_t)base);
+            const int64_t origin = scalar((int64_t)base);
 #pragma unroll
             for (int n = 0; n < chunks; ++n)
                 asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1"
                              :
-                             : "v"(at[n]), "s"(from), "s"(to + n * THREADS * 16)
+                             : "v"(from(n)), "s"(origin), "s"(to + n * THREADS * 16)
                              : "memory");
+        }
+        __device__ __forceinline__ void next(E* lds) {
+            send(lds, [&](int n) { return at[n]; });
             base += step;
+        }
+        // the last `left` of c, fewer than BK: what lies past them holds copies until cut() clears it
+        __device__ __forceinline__ void last(E* lds, int left) const {
+            send(lds, [&](int n) { return reach(n, left); });
+        }
+        static __device__ __forceinline__ void cut(E* lds, int left) {
+#pragma unroll 1
+            for (int n = 0; n < chunks; ++n) {
+                int idx, c;
+                place(threadIdx.x, n, idx, c);
+                if (c >= left) *reinterpret_cast<u32x4*>(lds + offset(idx, c)) = u32x4{};
+            }
         }
     };
 };
@@ -452,11 +497,13 @@ struct Product {
         multiply<T, TR, TB, BK, NR, NN>(lds, lds + P * TR::plane, wave / waves_n * WR, wave % waves_n * WN, acc);
     }
 
-    // acc += R[r0.., c] * B[n0.., c] over c in [c_lo, c_hi). `seen(stage of B)` is called on each stage.
+    // acc += R[r0.., c] * B[n0.., c] over c in [c_lo, c_hi). `seen(stage of B)` is called on each stage. r_end and
+    // b_end: the ends of the tensors.
     template <typename F>
     static __device__ __forceinline__ void run(E* s0, E* s1, f32x4 (&acc)[NR][NN], const T* r, int64_t r_pitch,
-                                               int64_t r0, int64_t r_n, const T* b, int64_t b_pitch,
-                                               int64_t n0, int64_t b_n, int64_t c_lo, int64_t c_hi, F&& seen) {
+                                               int64_t r0, int64_t r_n, const T* r_end, const T* b, int64_t b_pitch,
+                                               int64_t n0, int64_t b_n, const T* b_end, int64_t c_lo, int64_t c_hi,
+                                               F&& seen) {
         const int tid = threadIdx.x;
         if (c_lo >= c_hi) return;
         int64_t c = c_lo;
@@ -464,17 +511,26 @@ struct Product {
         const int full = __builtin_amdgcn_readfirstlane(whole ? (int)((c_hi - c_lo) / BK) : 0);
         c = c_lo + (int64_t)full * BK;
         if constexpr (DIRECT) {
-            if (full > 0) {
+            // a rest of c that cuts no piece goes the same way as the whole stages
+            const int rest = __builtin_amdgcn_readfirstlane(
+                whole && ((LR == ACROSS && LB == ACROSS) || (c_hi - c) % 8 == 0) ? (int)(c_hi - c) : 0);
+            const int stages = full + (rest > 0);
+            if (stages > 0) {
                 typename TR::Direct wr(r, r_pitch, r0, r_n, c_lo);
                 typename TB::Direct wb(b, b_pitch, n0, b_n, c_lo);
-                auto fill = [&](E* s) {
-                    wr.next(s);
-                    wb.next(s + TR::plane);
+                auto fill = [&](int k, E* s) {
+                    if (k < full) {
+                        wr.next(s);
+                        wb.next(s + TR::plane);
+                    } else {
+                        wr.last(s, rest);
+                        wb.last(s + TR::plane, rest);
+                    }
                 };
-                fill(s0);
+                fill(0, s0);
                 auto turn = [&](int k, E* now, E* next) {
                     arrive();  // stage `now` is filled, and nobody reads `next` any more
-                    if (k + 1 < full) fill(next);
+                    if (k + 1 < stages) fill(k + 1, next);
                     seen(now + TR::plane);
                     step(now, acc);
                 };
@@ -485,8 +541,18 @@ struct Product {
                 }
                 // (no exit from the middle of the loop: the accumulators would have a copy per exit)
                 if (k < full) turn(k, s0, s1);
+                if (rest > 0) {
+                    E* s = full % 2 ? s1 : s0;
+                    arrive();
+                    TR::Direct::cut(s, rest);
+                    TB::Direct::cut(s + TR::plane, rest);
+                    __syncthreads();
+                    seen(s + TR::plane);
+                    step(s, acc);
+                }
+                c += rest;
             }
-            for (; c < c_hi; c += BK) {  // what is left of c, and tiles at an end that cuts a piece
+            for (; c < c_hi; c += BK) {  // tiles at an end, or a rest of c, that cuts a piece
                 __syncthreads();
                 TR::copy(s0, tid, r, r_pitch, r0, r_n, c, c_hi);
                 TB::copy(s0 + TR::plane, tid, b, b_pitch, n0, b_n, c, c_hi);
@@ -518,8 +584,8 @@ struct Product {
                 }
             }
             for (; c < c_hi; c += BK) {
-                TR::load(rr, tid, r, r_pitch, r0, r_n, c, c_hi);
-                TB::load(rb, tid, b, b_pitch, n0, b_n, c, c_hi);
+                TR::load(rr, tid, r, r_pitch, r0, r_n, c, c_hi, r_end);
+                TB::load(rb, tid, b, b_pitch, n0, b_n, c, c_hi, b_end);
                 put();
                 seen(s0 + P * TR::plane);
                 step(s0, acc);
@@ -608,7 +674,8 @@ __device__ __forceinline__ void rows_tile(const GroupedArgs& a, const Item& it, 
     f32x4 acc[X::NR][X::NN] = {};
     const T* b = (const T*)a.b + (int64_t)it.group * a.b_group;
     if (it.group < a.groups)
-        X::run(s0, s1, acc, (const T*)a.r, a.r_pitch, r0, it.hi, b, a.b_pitch, n0, a.cols, 0, a.cc, [](auto*) {});
+        X::run(s0, s1, acc, (const T*)a.r, a.r_pitch, r0, it.hi, (const T*)a.r_end, b, a.b_pitch, n0, a.cols,
+               (const T*)a.b_end, 0, a.cc, [](auto*) {});
     if constexpr (sizeof(T) == 4) {
         if (it.group < a.groups && any_lost(acc)) {
 #pragma unroll
@@ -718,8 +785,8 @@ __global__ __launch_bounds__(WAVES * 64, 2) void grouped_few_rows_kernel(Grouped
             }
         }
         for (; c < c_hi; c += BK) {
-            TR::load(rr[0], lane, r, a.r_pitch, r0, it.hi, c, c_hi);
-            TB::load(rb[0], lane, b, a.b_pitch, n0, a.cols, c, c_hi);
+            TR::load(rr[0], lane, r, a.r_pitch, r0, it.hi, c, c_hi, (const T*)a.r_end);
+            TB::load(rb[0], lane, b, a.b_pitch, n0, a.cols, c, c_hi, (const T*)a.b_end);
             put(0);
             use();
         }
@@ -770,7 +837,8 @@ __global__ __launch_bounds__(THREADS, 2) void grouped_wgrad_kernel(GroupedArgs a
     const bool want_b = BIAS && r0 == 0;
     const T* r = (const T*)a.r;
     const T* b = (const T*)a.b;
-    X::run(s0, s1, acc, r, a.r_pitch, r0, a.out_rows, b, a.b_pitch, n0, a.cols, c_lo, c_hi, [&](auto* stage) {
+    X::run(s0, s1, acc, r, a.r_pitch, r0, a.out_rows, (const T*)a.r_end, b, a.b_pitch, n0, a.cols, (const T*)a.b_end, c_lo,
+           c_hi, [&](auto* stage) {
         if (!want_b) return;
 #pragma unroll
         for (int n = 0; n < X::TB::chunks; ++n) {
@@ -977,10 +1045,10 @@ int32_t rows_product(GroupedArgs a, hipStream_t strm) {
     const int64_t blocks = (a.rows / br + a.groups + 2) * a.col_tiles;
     if (blocks > INT32_MAX) return unsupported("grouped linear: more than 2^31 tiles");
     if (few) {
-        // workgroups that find rows: at most one per row and column tile; below two per CU a workgroup
-        // takes eight waves to have as many bytes on their way
+        // workgroups that find rows: at most one per row and column tile. Up to one per CU a workgroup takes
+        // eight waves, to have as many bytes on their way (of which a CU holds one workgroup, two of four)
         const int64_t busy = std::min<int64_t>(a.rows, a.rows / br + a.groups) * a.col_tiles;
-        if (busy < 512) launch_few<T, LB, 8>(a, (unsigned)blocks, strm);
+        if (busy <= 256) launch_few<T, LB, 8>(a, (unsigned)blocks, strm);
         else launch_few<T, LB, 4>(a, (unsigned)blocks, strm);
     } else if constexpr (sizeof(T) == 2) {
         if (big) launch_rows<T, LB, 256, 512, true>(a, (unsigned)blocks, strm);
@@ -995,6 +1063,10 @@ int32_t rows_product(GroupedArgs a, hipStream_t strm) {
 template <typename T>
 int32_t rows_either(const GroupedArgs& a, bool dgrad, hipStream_t strm) {
     return dgrad ? rows_product<T, ALONG>(a, strm) : rows_product<T, ACROSS>(a, strm);
+}
+
+const void* end_of(const void* p, int64_t rows, int64_t pitch, int64_t width, int32_t dtype) {
+    return rows < 1 ? p : (const char*)p + ((rows - 1) * pitch + width) * dtype_bytes(dtype);
 }
 
 int32_t rows_by_type(const GroupedArgs& a, int32_t dtype, bool dgrad, hipStream_t strm) {
@@ -1060,6 +1132,8 @@ extern "C" int32_t mpgnn_grouped_linear_fwd(const void* x, int64_t rows, int64_t
     a.r = x; a.r_pitch = x_pitch; a.b = weight; a.b_pitch = n; a.b_group = k * n; a.out = out; a.bias = bias;
     a.ptr = group_ptr; a.ptr64 = ptr_bits == 64; a.rows = rows; a.groups = (int32_t)groups; a.cc = (int32_t)k;
     a.cols = (int32_t)n;
+    a.r_end = end_of(x, rows, x_pitch, k, dtype);
+    a.b_end = end_of(weight, groups * k, n, n, dtype);
     return rows_by_type(a, dtype, false, static_cast<hipStream_t>(stream));
 }
 
@@ -1075,6 +1149,8 @@ extern "C" int32_t mpgnn_grouped_linear_dgrad(const void* dy, int64_t rows, int6
     a.r = dy; a.r_pitch = dy_pitch; a.b = weight; a.b_pitch = n; a.b_group = k * n; a.out = dx;
     a.ptr = group_ptr; a.ptr64 = ptr_bits == 64; a.rows = rows; a.groups = (int32_t)groups; a.cc = (int32_t)n;
     a.cols = (int32_t)k;
+    a.r_end = end_of(dy, rows, dy_pitch, n, dtype);
+    a.b_end = end_of(weight, groups * k, n, n, dtype);
     return rows_by_type(a, dtype, true, static_cast<hipStream_t>(stream));
 }
 
@@ -1109,6 +1185,8 @@ extern "C" int32_t mpgnn_grouped_linear_wgrad(const void* x, int64_t x_pitch, co
     a.r = x; a.r_pitch = x_pitch; a.b = dy; a.b_pitch = dy_pitch; a.out = dweight; a.dbias = dbias;
     a.slabs = static_cast<float*>(workspace); a.ptr = group_ptr; a.ptr64 = ptr_bits == 64; a.rows = rows;
     a.groups = (int32_t)groups; a.out_rows = (int32_t)k; a.cols = (int32_t)n; a.chunk = (int32_t)chunk;
+    a.r_end = end_of(x, rows, x_pitch, k, dtype);
+    a.b_end = end_of(dy, rows, dy_pitch, n, dtype);
     hipStream_t strm = static_cast<hipStream_t>(stream);
     if (dtype == MPGNN_F32) return wgrad_product<float>(a, strm);
     return dtype == MPGNN_BF16 ? wgrad_product<__bf16>(a, strm) : wgrad_product<_Float16>(a, strm);

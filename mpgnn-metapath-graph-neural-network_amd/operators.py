@@ -28,17 +28,18 @@ from .functional import _ptr, _stream_of
 __all__ = ["layer_norm", "grouped_linear", "clip_by_global_norm", "clip_grad_norm_"]
 
 _DTYPE = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
+_PTR_BITS = {torch.int64: 64, torch.int32: 32}
 
 
 def _require(t: torch.Tensor, name: str) -> int:
     """The mpgnn_dtype of a GPU tensor that the operators take."""
+    code = _DTYPE.get(t.dtype)
+    if code is not None and t.is_cuda:
+        return code
     if not t.is_cuda:
         raise RuntimeError(f"mpgnn_amd: `{name}` is on {t.device}; the operators run only as HIP kernels on a ROCm "
                            "GPU (there is no CPU fallback). Move the model and data to 'cuda'.")
-    code = _DTYPE.get(t.dtype)
-    if code is None:
-        raise TypeError(f"mpgnn_amd: `{name}` must be float32, bfloat16 or float16, got {t.dtype}")
-    return code
+    raise TypeError(f"mpgnn_amd: `{name}` must be float32, bfloat16 or float16, got {t.dtype}")
 
 
 def _call(device: torch.device, entry, *args) -> None:
@@ -82,25 +83,30 @@ def _once(backward):
 def _rows_view(t: torch.Tensor) -> tuple[torch.Tensor, int, int]:
     """(tensor, rows, row pitch) of t as rows of its last dimension: t itself where its rows lie a
     constant pitch apart (contiguous, or a column slice of a matrix), else a contiguous copy."""
-    width = t.shape[-1]
-    rows = t.numel() // width
-    if t.is_contiguous():
-        return t, rows, width
-    if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= width:
-        return t, rows, t.stride(0)
-    return t.contiguous(), rows, width
+    shape = t.shape
+    width = shape[-1]
+    rows = shape[0] if len(shape) == 2 else t.numel() // width
+    if not t.is_contiguous():
+        if len(shape) == 2:
+            pitch, inner = t.stride()
+            if inner == 1 and pitch >= width:
+                return t, rows, pitch
+        t = t.contiguous()
+    return t, rows, width
 
 
 def _norm_forward(x, weight, bias, eps, code, wcode, keep):
     xr, rows, pitch = _rows_view(x)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if keep else None
-    mean = rstd = None
+    device = x.device
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    stats = mean = rstd = None
     if keep:
+        stats = torch.empty((2, rows), dtype=torch.float32, device=device)
         mean = stats.data_ptr()
         rstd = mean + 4 * rows
-    _call(x.device, lib.mpgnn_layer_norm_fwd, xr.data_ptr(), rows, x.shape[-1], pitch, code, _ptr(weight), _ptr(bias),
-          wcode, eps, y.data_ptr(), mean, rstd)
+    _call(device, lib.mpgnn_layer_norm_fwd, xr.data_ptr(), rows, x.shape[-1], pitch, code,
+          None if weight is None else weight.data_ptr(), None if bias is None else bias.data_ptr(), wcode, eps,
+          y.data_ptr(), mean, rstd)
     return y, xr, stats
 
 
@@ -145,31 +151,38 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor = None, bias: torch.Tensor 
 
     ``weight`` / ``bias``: [x.shape[-1]], of x's type or both fp32, or None. A column slice of a
     matrix is read in place. Differentiable once in x, weight and bias."""
-    code = _require(x, "x")
-    if x.dim() == 0 or x.shape[-1] == 0:
-        raise ValueError(f"layer_norm normalises a last dimension of at least one element, got shape {tuple(x.shape)}")
-    wcode = code
-    for name, p in (("weight", weight), ("bias", bias)):
-        if p is None:
-            continue
-        c = _require(p, name)
-        if p.dim() != 1 or p.shape[0] != x.shape[-1]:
-            raise ValueError(f"`{name}` has shape {tuple(p.shape)}, expected ({x.shape[-1]},)")
-        if p.device != x.device:
-            raise RuntimeError(f"`{name}` is on {p.device}, x on {x.device}")
-        if c != code and c != F32:
-            raise TypeError(f"`{name}` must be {x.dtype} or float32, got {p.dtype}")
+    code = wcode = _require(x, "x")
+    shape = x.shape
+    if not shape or shape[-1] == 0:
+        raise ValueError(f"layer_norm normalises a last dimension of at least one element, got shape {tuple(shape)}")
+    grad = x.requires_grad
+    if weight is not None:
+        wcode = _check_param(weight, "weight", x, shape[-1], code)
+        grad = grad or weight.requires_grad
+        if not weight.is_contiguous():
+            weight = weight.contiguous()
+    if bias is not None:
+        c = _check_param(bias, "bias", x, shape[-1], code)
+        if weight is not None and c != wcode:
+            raise TypeError(f"weight and bias must have one type, got {weight.dtype} and {bias.dtype}")
         wcode = c
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise TypeError(f"weight and bias must have one type, got {weight.dtype} and {bias.dtype}")
-    if weight is not None and not weight.is_contiguous():
-        weight = weight.contiguous()
-    if bias is not None and not bias.is_contiguous():
-        bias = bias.contiguous()
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
-                                    or (bias is not None and bias.requires_grad)):
+        grad = grad or bias.requires_grad
+        if not bias.is_contiguous():
+            bias = bias.contiguous()
+    if grad and torch.is_grad_enabled():
         return _LayerNormFn.apply(x, weight, bias, float(eps), code, wcode)
     return _norm_forward(x, weight, bias, float(eps), code, wcode, False)[0]
+
+
+def _check_param(p, name, x, width, code) -> int:
+    c = _require(p, name)
+    if p.shape != (width,):
+        raise ValueError(f"`{name}` has shape {tuple(p.shape)}, expected ({width},)")
+    if p.get_device() != x.get_device():
+        raise RuntimeError(f"`{name}` is on {p.device}, x on {x.device}")
+    if c != code and c != F32:
+        raise TypeError(f"`{name}` must be {x.dtype} or float32, got {p.dtype}")
+    return c
 
 
 # ---------------------------------------------------------------------------------------
@@ -230,36 +243,43 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, group_ptr: torch.Tenso
     Groups may be empty. Rows before ``group_ptr[0]`` or from ``group_ptr[-1]`` on belong to no group: their
     output and gradient rows are zero. Differentiable once in x, weight and bias."""
     code = _require(x, "x")
-    if x.dim() != 2 or weight.dim() != 3 or group_ptr.dim() != 1:
+    sx, sw, sp = x.shape, weight.shape, group_ptr.shape
+    if len(sx) != 2 or len(sw) != 3 or len(sp) != 1:
         raise ValueError("grouped_linear takes x [rows, K], weight [groups, K, N] and group_ptr [groups + 1], got "
-                         f"{tuple(x.shape)}, {tuple(weight.shape)} and {tuple(group_ptr.shape)}")
-    groups, k, n = weight.shape
+                         f"{tuple(sx)}, {tuple(sw)} and {tuple(sp)}")
+    groups, k, n = sw
     if groups < 1 or k < 1 or n < 1:
-        raise ValueError(f"grouped_linear needs at least one group, input and output column, got weight {tuple(weight.shape)}")
-    if x.shape[1] != k:
-        raise RuntimeError(f"mat1 and mat2 shapes cannot be multiplied ({x.shape[0]}x{x.shape[1]} and {k}x{n})")
-    if group_ptr.shape[0] != groups + 1:
-        raise ValueError(f"group_ptr has {group_ptr.shape[0]} entries, expected groups + 1 = {groups + 1}")
-    if group_ptr.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"grouped_linear needs at least one group, input and output column, got weight {tuple(sw)}")
+    if sx[1] != k:
+        raise RuntimeError(f"mat1 and mat2 shapes cannot be multiplied ({sx[0]}x{sx[1]} and {k}x{n})")
+    if sp[0] != groups + 1:
+        raise ValueError(f"group_ptr has {sp[0]} entries, expected groups + 1 = {groups + 1}")
+    bits = _PTR_BITS.get(group_ptr.dtype)
+    if bits is None:
         raise TypeError(f"group_ptr must be int32 or int64, got {group_ptr.dtype}")
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is None:
-            continue
-        if _require(t, name) != code:
-            raise TypeError(f"`{name}` must be {x.dtype} as x is, got {t.dtype}")
-        if t.device != x.device:
-            raise RuntimeError(f"`{name}` is on {t.device}, x on {x.device}")
-    if group_ptr.device != x.device:
+    where = x.get_device()
+    if _require(weight, "weight") != code:
+        raise TypeError(f"`weight` must be {x.dtype} as x is, got {weight.dtype}")
+    if weight.get_device() != where:
+        raise RuntimeError(f"`weight` is on {weight.device}, x on {x.device}")
+    if group_ptr.get_device() != where:
         raise RuntimeError(f"`group_ptr` is on {group_ptr.device}, x on {x.device}")
-    if bias is not None and tuple(bias.shape) != (groups, n):
-        raise ValueError(f"bias has shape {tuple(bias.shape)}, expected {(groups, n)}")
-    ptr = group_ptr if group_ptr.is_contiguous() else group_ptr.contiguous()
-    bits = 64 if ptr.dtype == torch.int64 else 32
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
-        return _GroupedLinearFn.apply(x, weight, bias, ptr, bits, code)
+    grad = x.requires_grad or weight.requires_grad
+    if bias is not None:
+        if _require(bias, "bias") != code:
+            raise TypeError(f"`bias` must be {x.dtype} as x is, got {bias.dtype}")
+        if bias.get_device() != where:
+            raise RuntimeError(f"`bias` is on {bias.device}, x on {x.device}")
+        if bias.shape != (groups, n):
+            raise ValueError(f"bias has shape {tuple(bias.shape)}, expected {(groups, n)}")
+        grad = grad or bias.requires_grad
+    if not group_ptr.is_contiguous():
+        group_ptr = group_ptr.contiguous()
+    if grad and torch.is_grad_enabled():
+        return _GroupedLinearFn.apply(x, weight, bias, group_ptr, bits, code)
     xr, _, pitch = _rows_view(x)
     return _grouped_forward(xr, pitch, weight if weight.is_contiguous() else weight.contiguous(),
-                            bias if bias is None or bias.is_contiguous() else bias.contiguous(), ptr, bits, code)
+                            bias if bias is None or bias.is_contiguous() else bias.contiguous(), group_ptr, bits, code)
 
 
 # ---------------------------------------------------------------------------------------
