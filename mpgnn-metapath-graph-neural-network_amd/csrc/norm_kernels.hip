@@ -118,36 +118,68 @@ struct RowShape {
 };
 
 // A thread's part of a row on its way from memory: the next row is asked for before the current
-// one's sums, whose barriers it does not wait for.
-template <typename T, int V, int TPR, int NV>
+// one's sums, whose barriers it does not wait for. WHOLE: rows of whole 16-byte vectors at multiples of 16
+// bytes. Else vectors start where they may (the hardware's loads need no more than an element's alignment),
+// and the one that the end of the row cuts goes element by element.
+template <typename T, int V, int TPR, int NV, bool WHOLE>
 struct Row {
-    typename VecOf<T, V>::type v[NV];
+    typedef typename VecOf<T, V>::type Vec;
+    Vec v[NV];
 
     __device__ __forceinline__ void load(const T* p, int64_t pitch, int64_t r, int64_t rows, int t, int F) {
         const bool live = r < rows;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (i * TPR + t) * V;
-            v[i] = live && c < F ? *reinterpret_cast<const typename VecOf<T, V>::type*>(p + r * pitch + c)
-                                 : typename VecOf<T, V>::type(0);
+            const T* at = p + r * pitch + c;
+            v[i] = Vec(0);
+            if (!live) continue;
+            if constexpr (WHOLE) {
+                if (c < F) v[i] = *reinterpret_cast<const Vec*>(at);
+            } else if (c + V <= F) {
+                __builtin_memcpy(&v[i], at, sizeof(Vec));
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    if (c + j < F) v[i][j] = at[j];
+            }
         }
     }
     __device__ __forceinline__ void widen(float (&f)[NV][V]) const {
 #pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j) f[i][j] = (float)v[i][j];
+    }
+    static __device__ __forceinline__ void store(T* p, const float (&f)[NV][V], int t, int F) {
+#pragma unroll
         for (int i = 0; i < NV; ++i) {
-            if constexpr (V == 1) {
-                f[i][0] = (float)v[i];
+            const int c = (i * TPR + t) * V;
+            if (c >= F) continue;
+            Vec o;
+#pragma unroll
+            for (int j = 0; j < V; ++j) o[j] = (T)f[i][j];
+            if constexpr (WHOLE) {
+                *reinterpret_cast<Vec*>(p + c) = o;
+            } else if (c + V <= F) {
+                __builtin_memcpy(p + c, &o, sizeof(Vec));
             } else {
 #pragma unroll
-                for (int j = 0; j < V; ++j) f[i][j] = (float)v[i][j];
+                for (int j = 0; j < V; ++j)
+                    if (c + j < F) p[c + j] = o[j];
             }
         }
     }
+    // is element j of a thread's vector i inside the row?
+    static __device__ __forceinline__ bool in(int i, int j, int t, int F) {
+        return (i * TPR + t) * V + (WHOLE ? 0 : j) < F;
+    }
 };
 
-template <typename T, int V, int TPR, int NV>
+template <typename T, int V, int TPR, int NV, bool WHOLE>
 __global__ __launch_bounds__(RowShape<TPR>::threads) void layer_norm_fwd_kernel(NormArgs a) {
     using S = RowShape<TPR>;
+    using R = Row<T, V, TPR, NV, WHOLE>;
     __shared__ float lds[S::lds];
     const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
     const int F = a.width;
@@ -164,7 +196,7 @@ __global__ __launch_bounds__(RowShape<TPR>::threads) void layer_norm_fwd_kernel(
     const bool full = F == TPR * NV * V;
     int turn = 0;
     const int64_t step = (int64_t)gridDim.x * S::rows;
-    Row<T, V, TPR, NV> next;
+    R next;
     next.load((const T*)a.x, a.x_pitch, (int64_t)blockIdx.x * S::rows + sub, a.rows, t, F);
     // every thread of the workgroup takes part in each turn's sums; rows past the end are not touched
     for (int64_t r0 = (int64_t)blockIdx.x * S::rows; r0 < a.rows; r0 += step) {
@@ -194,27 +226,21 @@ __global__ __launch_bounds__(RowShape<TPR>::threads) void layer_norm_fwd_kernel(
             row_sum<TPR, 1>(s, lds, turn);
             mean = s[0] / width;
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const bool in = (i * TPR + t) * V < F;
+            for (int i = 0; i < NV; ++i)
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
                     v[i][j] -= mean;
-                    if (in) q[0] = __builtin_fmaf(v[i][j], v[i][j], q[0]);
+                    if (R::in(i, j, t, F)) q[0] = __builtin_fmaf(v[i][j], v[i][j], q[0]);
                 }
-            }
             row_sum<TPR, 1>(q, lds, turn);
         }
         const float rstd = 1.0f / sqrtf(q[0] / width + a.eps);
         if (!live) continue;
-        T* y = (T*)a.out + r * F;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (i * TPR + t) * V;
-            if (c >= F) continue;
+        for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int j = 0; j < V; ++j) v[i][j] = __builtin_fmaf(v[i][j] * rstd, w[i][j], b[i][j]);
-            store_vec<T, V>(y + c, v[i]);
-        }
+        R::store((T*)a.out + r * F, v, t, F);
         if (a.mean && t == 0) {
             a.mean[r] = mean;
             a.rstd[r] = rstd;
@@ -236,9 +262,10 @@ __device__ __forceinline__ void add_to(float& a, float& c, float v) {
     }
 }
 
-template <typename T, int V, int TPR, int NV>
+template <typename T, int V, int TPR, int NV, bool WHOLE>
 __global__ __launch_bounds__(RowShape<TPR>::threads) void layer_norm_bwd_kernel(NormArgs a) {
     using S = RowShape<TPR>;
+    using R = Row<T, V, TPR, NV, WHOLE>;
     constexpr bool COMP = sizeof(T) == 4;
     constexpr int COLS = TPR * NV * V;
     __shared__ float lds[S::lds];
@@ -260,7 +287,7 @@ __global__ __launch_bounds__(RowShape<TPR>::threads) void layer_norm_bwd_kernel(
     const float width = (float)F;
     int turn = 0;
     const int64_t step = (int64_t)gridDim.x * S::rows;
-    Row<T, V, TPR, NV> next_x, next_dy;
+    R next_x, next_dy;
     float next_mean = 0.0f, next_rstd = 0.0f;
     auto fetch = [&](int64_t r) {
         next_x.load((const T*)a.x, a.x_pitch, r, a.rows, t, F);
@@ -280,11 +307,10 @@ __global__ __launch_bounds__(RowShape<TPR>::threads) void layer_norm_bwd_kernel(
         next_dy.widen(g);
         fetch(r + step);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const bool in = live && (i * TPR + t) * V < F;
+        for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                if (!in) continue;
+                if (!(live && R::in(i, j, t, F))) continue;
                 xh[i][j] = (xh[i][j] - mean) * rstd;
                 add_to<COMP>(dw[i][j], dwc[COMP ? i : 0][j], g[i][j] * xh[i][j]);
                 add_to<COMP>(db[i][j], dbc[COMP ? i : 0][j], g[i][j]);
@@ -292,20 +318,15 @@ __global__ __launch_bounds__(RowShape<TPR>::threads) void layer_norm_bwd_kernel(
                 s[0] += g[i][j];
                 s[1] = __builtin_fmaf(g[i][j], xh[i][j], s[1]);
             }
-        }
         if (!a.out) continue;
         row_sum<TPR, 2>(s, lds, turn);
         if (!live) continue;
         const float m1 = s[0] / width, m2 = s[1] / width;
-        T* dx = (T*)a.out + r * F;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (i * TPR + t) * V;
-            if (c >= F) continue;
+        for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int j = 0; j < V; ++j) g[i][j] = rstd * (g[i][j] - m1 - xh[i][j] * m2);
-            store_vec<T, V>(dx + c, g[i]);
-        }
+        R::store((T*)a.out + r * F, g, t, F);
     }
     if (!a.part) return;
     // one partial row per workgroup: its row slots added in order through LDS
@@ -441,31 +462,32 @@ __global__ __launch_bounds__(1024) void layer_norm_reduce_kernel(const float* pa
 // and read once in fp32, are at most a tenth of the traffic of x, dy and dx.
 int64_t norm_partials(int64_t rows, int eb) { return std::max<int64_t>(256, std::min<int64_t>(2048, rows * eb / 54)); }
 
-template <typename T, int V, int TPR, int NV>
+template <typename T, int TPR, int NV, bool WHOLE>
 void launch_rows(const NormArgs& a, bool bwd, int max_blocks, hipStream_t strm) {
     using S = RowShape<TPR>;
+    constexpr int V = 16 / sizeof(T);
     const int blocks = (int)std::min<int64_t>(max_blocks, (a.rows + S::rows - 1) / S::rows);
     if (bwd)
-        hipLaunchKernelGGL((layer_norm_bwd_kernel<T, V, TPR, NV>), dim3(blocks), dim3(S::threads), 0, strm, a);
+        hipLaunchKernelGGL((layer_norm_bwd_kernel<T, V, TPR, NV, WHOLE>), dim3(blocks), dim3(S::threads), 0, strm, a);
     else
-        hipLaunchKernelGGL((layer_norm_fwd_kernel<T, V, TPR, NV>), dim3(blocks), dim3(S::threads), 0, strm, a);
+        hipLaunchKernelGGL((layer_norm_fwd_kernel<T, V, TPR, NV, WHOLE>), dim3(blocks), dim3(S::threads), 0, strm, a);
 }
 
-// The narrowest team of threads that holds a row of `vecs` vectors; false: none does.
-template <typename T, int V>
-bool launch_by_width(const NormArgs& a, bool bwd, int max_blocks, hipStream_t strm) {
-    const int vecs = (a.width + V - 1) / V;
-    if (vecs <= 16) launch_rows<T, V, 16, 1>(a, bwd, max_blocks, strm);
-    else if (vecs <= 32) launch_rows<T, V, 32, 1>(a, bwd, max_blocks, strm);
-    else if (vecs <= 64) launch_rows<T, V, 64, 1>(a, bwd, max_blocks, strm);
-    else if (vecs <= 128) launch_rows<T, V, 64, 2>(a, bwd, max_blocks, strm);
-    else if (vecs <= 256) launch_rows<T, V, 256, 1>(a, bwd, max_blocks, strm);
-    else if (vecs <= 512) launch_rows<T, V, 256, 2>(a, bwd, max_blocks, strm);
-    else if (vecs <= 1024) launch_rows<T, V, 256, 4>(a, bwd, max_blocks, strm);
-    else if (vecs <= 2048) launch_rows<T, V, 1024, 2>(a, bwd, max_blocks, strm);
-    else return false;
-    return true;
+// The narrowest team of threads that holds a row of `vecs` vectors, at most 2,048.
+template <typename T, bool WHOLE>
+void launch_by_width(const NormArgs& a, int vecs, bool bwd, int max_blocks, hipStream_t strm) {
+    if (vecs <= 16) launch_rows<T, 16, 1, WHOLE>(a, bwd, max_blocks, strm);
+    else if (vecs <= 32) launch_rows<T, 32, 1, WHOLE>(a, bwd, max_blocks, strm);
+    else if (vecs <= 64) launch_rows<T, 64, 1, WHOLE>(a, bwd, max_blocks, strm);
+    else if (vecs <= 128) launch_rows<T, 64, 2, WHOLE>(a, bwd, max_blocks, strm);
+    else if (vecs <= 256) launch_rows<T, 256, 1, WHOLE>(a, bwd, max_blocks, strm);
+    else if (vecs <= 512) launch_rows<T, 256, 2, WHOLE>(a, bwd, max_blocks, strm);
+    else if (vecs <= 1024) launch_rows<T, 256, 4, WHOLE>(a, bwd, max_blocks, strm);
+    else launch_rows<T, 1024, 2, WHOLE>(a, bwd, max_blocks, strm);
 }
+
+template <typename T>
+int row_vecs(const NormArgs& a) { return (a.width + 16 / (int)sizeof(T) - 1) / (16 / (int)sizeof(T)); }
 
 bool vec_ok(const NormArgs& a, int eb) {
     const int v = 16 / eb;
@@ -476,11 +498,14 @@ bool vec_ok(const NormArgs& a, int eb) {
 template <typename T>
 int32_t norm_fwd(const NormArgs& a, hipStream_t strm) {
     constexpr int max_blocks = 256 * 8;
-    const bool done = vec_ok(a, sizeof(T)) ? launch_by_width<T, 16 / sizeof(T)>(a, false, max_blocks, strm)
-                                           : launch_by_width<T, 1>(a, false, max_blocks, strm);
-    if (!done)
+    const int vecs = row_vecs<T>(a);
+    if (vecs <= 2048) {
+        if (vec_ok(a, sizeof(T))) launch_by_width<T, true>(a, vecs, false, max_blocks, strm);
+        else launch_by_width<T, false>(a, vecs, false, max_blocks, strm);
+    } else {
         hipLaunchKernelGGL(layer_norm_fwd_wide_kernel<T>, dim3((unsigned)std::min<int64_t>(a.rows, 1024)), dim3(kWide),
                            0, strm, a);
+    }
     return launch_status("mpgnn_layer_norm_fwd: the launch failed");
 }
 
@@ -488,14 +513,13 @@ template <typename T>
 int32_t norm_bwd(const NormArgs& a, void* dw, void* db, hipStream_t strm) {
     int parts = 0;
     const int max_parts = (int)norm_partials(a.rows, sizeof(T));
-    const int V = vec_ok(a, sizeof(T)) ? 16 / (int)sizeof(T) : 1;
-    const int vecs = (a.width + V - 1) / V;
+    const int vecs = row_vecs<T>(a);
     const int rows_per = vecs <= 16 ? 16 : vecs <= 32 ? 8 : vecs <= 128 ? 4 : 1;
     if (a.rows == 0) {  // no partial rows: the parameters' gradients are zero
     } else if (vecs <= 2048) {
         parts = (int)std::min<int64_t>(max_parts, (a.rows + rows_per - 1) / rows_per);
-        if (V == 1) launch_by_width<T, 1>(a, true, max_parts, strm);
-        else launch_by_width<T, 16 / sizeof(T)>(a, true, max_parts, strm);
+        if (vec_ok(a, sizeof(T))) launch_by_width<T, true>(a, vecs, true, max_parts, strm);
+        else launch_by_width<T, false>(a, vecs, true, max_parts, strm);
     } else {
         if (a.out)
             hipLaunchKernelGGL(layer_norm_bwd_wide_kernel<T>, dim3((unsigned)std::min<int64_t>(a.rows, 1024)),

@@ -17,31 +17,18 @@ template <typename T, int V>
 struct VecOf {
     typedef T type __attribute__((ext_vector_type(V)));
 };
-template <typename T>
-struct VecOf<T, 1> {
-    typedef T type;
-};
-
 template <typename T, int V>
 __device__ __forceinline__ void load_vec(float (&dst)[V], const T* p) {
     const typename VecOf<T, V>::type v = *reinterpret_cast<const typename VecOf<T, V>::type*>(p);
-    if constexpr (V == 1) {
-        dst[0] = (float)v;
-    } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) dst[i] = (float)v[i];
-    }
+    for (int i = 0; i < V; ++i) dst[i] = (float)v[i];
 }
 
 template <typename T, int V>
 __device__ __forceinline__ void store_vec(T* p, const float (&src)[V]) {
     typename VecOf<T, V>::type v;
-    if constexpr (V == 1) {
-        v = (T)src[0];
-    } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = (T)src[i];
-    }
+    for (int i = 0; i < V; ++i) v[i] = (T)src[i];
     *reinterpret_cast<typename VecOf<T, V>::type*>(p) = v;
 }
 
