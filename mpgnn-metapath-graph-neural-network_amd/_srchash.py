@@ -1,4 +1,4 @@
-"""Source hash of libmpgnn_rgcn.so (no package imports: __graft_entry__.build() loads this file
+"""Source hash of libmpgnn_rgcn.so and _operators.so (no package imports: __graft_entry__.build() loads this file
 by path before the library exists). build() writes it next to the library; _lib.py refuses a
 library whose stamp does not match the sources in the tree."""
 import hashlib
@@ -7,7 +7,8 @@ import os
 HERE = os.path.dirname(os.path.abspath(__file__))
 SOURCES = ("csrc/Makefile", "csrc/plan.cpp", "csrc/plan_internal.h", "csrc/io.cpp", "csrc/rgcn_kernels.hip",
            "csrc/plan_device.hip", "csrc/score_kernels.hip", "csrc/optim_kernels.hip",
-           "csrc/norm_kernels.hip", "csrc/clip_kernels.hip", "csrc/grouped_kernels.hip", "csrc/num_types.h", "../include/mpgnn_rgcn.h")
+           "csrc/norm_kernels.hip", "csrc/clip_kernels.hip", "csrc/grouped_kernels.hip", "csrc/num_types.h",
+           "csrc/operators_torch.cpp", "../include/mpgnn_rgcn.h")
 STAMP = os.path.join(HERE, "libmpgnn_rgcn.so.srchash")
 
 

@@ -760,3 +760,32 @@ def test_wrong_ptr_stays_inside_the_tensors():
         clamped = [min(max(v, 0), 64) for v in vals]
         ref, mag = gl_reference(x.cpu(), w.cpu(), None, clamped)
         within(y, ref, gl_tol(ref, mag, 32, torch.float32), vals)
+
+
+def test_graphs_of_the_backward():
+    """No second derivative by any argument, also where the incoming gradient is a constant; a graph is
+    run once unless it is kept; a saved tensor that is written to is noticed."""
+    g = gen(77)
+    x, w = rnd(g, 6, 8).to(DEV).requires_grad_(True), rnd(g, 2, 8, 5).to(DEV).requires_grad_(True)
+    ptr = torch.tensor([0, 2, 6], device=DEV)
+    for f in (lambda t: mpgnn_amd.layer_norm(t), lambda t: mpgnn_amd.grouped_linear(t, w, ptr)):
+        first = torch.autograd.grad(f(x).sum(), x)[0]
+        gx = torch.autograd.grad(f(x).sum(), x, create_graph=True)[0]
+        assert torch.equal(gx.detach(), first)
+        with pytest.raises(RuntimeError, match="second derivative"):
+            (gx * gx).sum().backward()
+        y = f(x)
+        for _ in range(2):
+            assert torch.equal(torch.autograd.grad(y.sum(), x, retain_graph=True)[0], first)
+        torch.autograd.grad(y.sum(), x)
+        with pytest.raises(RuntimeError, match="second time"):
+            torch.autograd.grad(y.sum(), x)
+        z = x * 1.0
+        y = f(z)
+        z.mul_(2.0)
+        with pytest.raises(RuntimeError, match="inplace"):
+            y.sum().backward()
+    # the graph of another argument only
+    y = mpgnn_amd.grouped_linear(x.detach(), w, ptr)
+    dw = torch.autograd.grad(y.sum(), w)[0]
+    assert torch.equal(dw, torch.autograd.grad(mpgnn_amd.grouped_linear(x, w, ptr).sum(), w)[0])
