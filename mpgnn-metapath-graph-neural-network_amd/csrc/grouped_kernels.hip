@@ -60,6 +60,7 @@ struct GroupedArgs {
     int32_t col_tiles, row_tiles;
     int32_t chunk;      // weight gradient: rows of a chunk
     int64_t items;      // weight gradient: slabs there are room for
+    int32_t run;        // tiles that an XCD takes in a row
 };
 
 // 8 values of c of one index from a tile stored across: two transposed reads of 4 c x 16 indices
@@ -111,6 +112,13 @@ __device__ __forceinline__ int64_t ptr_at(const GroupedArgs& a, int g) {
 __device__ __forceinline__ int64_t scalar(int64_t v) {
     return (int64_t)((uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 |
                      (unsigned)__builtin_amdgcn_readfirstlane((int)v));
+}
+
+// The tile of this workgroup. Workgroups go to the eight XCDs in turn, each of which has an L2 of its own: an
+// XCD takes `run` tiles in a row, so that tiles which read the same rows read them from memory once.
+__device__ __forceinline__ int tile_of(const GroupedArgs& a) {
+    const unsigned id = blockIdx.x, run = a.run;
+    return (int)(id / (8 * run) * (8 * run) + id % 8 * run + id / 8 % run);
 }
 
 struct Item {
@@ -710,9 +718,10 @@ __global__ __launch_bounds__(THREADS, 2) void grouped_rows_kernel(GroupedArgs a)
     typedef Product<T, ALONG, LB, BR, BN, THREADS, DIRECT> X;
     __shared__ __attribute__((aligned(16))) typename X::E s0[X::stage];
     __shared__ __attribute__((aligned(16))) typename X::E s1[DIRECT ? X::stage : 8];
-    const Item it = find_item<THREADS>(a, blockIdx.x / a.col_tiles, BR, 0, true);
+    const int bid = tile_of(a);
+    const Item it = find_item<THREADS>(a, bid / a.col_tiles, BR, 0, true);
     if (it.group < 0) return;
-    const int64_t n0 = (int64_t)(blockIdx.x % a.col_tiles) * BN;
+    const int64_t n0 = (int64_t)(bid % a.col_tiles) * BN;
     const int64_t r0 = it.lo + (int64_t)it.part * BR;
     if constexpr (BR == 256) {
         if (it.hi - r0 <= BR / 2) {
@@ -825,8 +834,8 @@ __global__ __launch_bounds__(THREADS, 2) void grouped_wgrad_kernel(GroupedArgs a
     __shared__ __attribute__((aligned(16))) typename X::E s0[X::stage];
     __shared__ __attribute__((aligned(16))) typename X::E s1[DIRECT ? X::stage : 8];
     const int tiles = a.row_tiles * a.col_tiles;
-    const int id = blockIdx.x / tiles;
-    const int tile = blockIdx.x % tiles;
+    const int bid = tile_of(a);
+    const int id = bid / tiles, tile = bid % tiles;
     const Item it = find_item<THREADS>(a, id, a.chunk, 1, false);
     if (it.group < 0) return;
     const int64_t r0 = (int64_t)(tile / a.col_tiles) * BR, n0 = (int64_t)(tile % a.col_tiles) * BN;
@@ -978,23 +987,30 @@ constexpr int kTile = 128;
 // Tiles of 256 x 256 read half as many bytes a product as tiles of 128 x 128, which the CUs' 64 bytes a
 // clock from L2 hold to half the matrix rate; but a CU has one at a time, so that they need rounds
 // enough: bf16, us for forward / input / weight gradient with 128 and 256:
-//   32768 rows, 32 groups, 2048 x 4096   745 / 650 / 896    591 / 582 / 720
-//   32768 rows, 128 groups, 1024 x 2048  245 / 243 / 466    239 / 223 / 392
-//   16384 rows, 4 groups, 1024 x 1024     63 /  63 /  92     67 /  65 /  97
-//   8192 rows, 8 groups, 512 x 2048       36 /  36 /  65     46 /  51 /  72
-constexpr int64_t kBigTiles = 512;
-constexpr int kFewRows = 32;  // rows a group on average, up to which grouped_few_rows_kernel runs
+//   32768 rows, 32 groups, 2048 x 4096   695 / 657 / 802    535 / 502 / 622
+//   24576 rows, 8 groups, 1024 x 1024     73 /  81 /  74     70 /  70 /  74
+//   20480 rows, 4 groups, 1024 x 1024     62 /  62 /  86     68 /  67 /  86
+constexpr int64_t kBigTiles = 384;
+// Up to this many rows a group on average grouped_few_rows_kernel runs, and up to this many of its tiles: larger
+// tiles would leave most CUs idle, each with all of c to go through. us with tiles of 128 x 128 and with these, one
+// group:
+//   bf16, 512 rows, 2048 x 2048    24 / 16       fp32    86 / 45    (512 tiles of 32 x 64)
+//   bf16, 2048 rows, 2048 x 256    23 / 11               86 / 28    (256)
+//   bf16, 512 rows, 256 x 2048    7.9 / 7.7            16.5 / 11.7  (512)
+//   bf16, 8192 rows, 256 x 256      8 / 13               18 / 21    (1024)
+constexpr int kFewRows = 32, kFewTiles = 512;
 
 // Rows of a chunk of the weight gradient: whole groups where the weight alone has tiles enough to
 // fill the chip, else as many rows as leave two workgroups per CU (more chunks are more slabs to write and
-// add: 208k rows, 237 groups, 128 x 128 bf16 41 us, 48 with four). With many tiles of fp32, whose workgroups
+// add: 208k rows, 237 groups, 128 x 128 bf16 39 us, 48 with four), and no fewer than 256 (128 of fp32: 2725 rows, 3
+// groups, 216 x 256 16 us, 22 with 256). With many tiles of fp32, whose workgroups
 // run longer, uneven groups want four (20k rows, 8 groups, 1024 x 1024: 272 us, 342 with two).
 int64_t wgrad_chunk(int64_t rows, int64_t groups, int64_t k, int64_t n, int eb) {
     const int64_t tiles = ((k + kTile - 1) / kTile) * ((n + kTile - 1) / kTile);
     const int64_t want = (eb == 4 && tiles > 4 ? 1024 : 512) / tiles;  // chunks over all groups
     if (want <= groups || rows == 0) return std::max<int64_t>(rows, 1);
     const int64_t c = (rows + want - 1) / want;
-    return std::max<int64_t>(256, (c + 63) / 64 * 64);
+    return std::max<int64_t>(eb == 4 ? 128 : 256, (c + 63) / 64 * 64);
 }
 
 int64_t wgrad_items(int64_t rows, int64_t groups, int64_t chunk) { return rows / chunk + groups; }
@@ -1028,12 +1044,25 @@ void launch_rows(GroupedArgs a, unsigned blocks, hipStream_t strm) {
                        a);
 }
 
+// GroupedArgs::run for `blocks` tiles of which `sharing` in a row read the same rows, but no more than leave each
+// XCD eight runs of the `sure` tiles that there are whatever the groups' sizes. Returns the blocks to launch, whole
+// turns over the XCDs. Forward / input gradient in us with runs of one tile and with these:
+//   24k rows, 1 group, 1041 x 962 fp16     139 / 114    126 /  91
+//   56k rows, 32 groups, 3120 x 584 fp16   435 / 388    354 / 351
+//   262k rows, 19 groups, 168 x 792 fp16   324 / 184    256 / 184
+int64_t set_run(GroupedArgs& a, int64_t blocks, int64_t sharing, int64_t sure) {
+    a.run = (int32_t)std::max<int64_t>(1, std::min(sharing, sure / 64));
+    const int64_t turn = 8 * (int64_t)a.run;
+    return (blocks + turn - 1) / turn * turn;
+}
+
 // columns that tiles of 256 cover without much more padding than tiles of 128
 bool big_cols(int64_t n) { return n % 256 == 0 || n % 256 > 128 || n >= 1024; }
 
 template <typename T, Layout LB>
 int32_t rows_product(GroupedArgs a, hipStream_t strm) {
-    const bool few = a.rows <= (int64_t)kFewRows * a.groups;
+    const bool few = a.rows <= (int64_t)kFewRows * a.groups ||
+                     (a.rows / 32 * ((a.cols + 63) / 64) <= kFewTiles && (sizeof(T) == 4 || a.cc > 128));
     bool direct = false, big = false;
     if constexpr (sizeof(T) == 2) {
         direct = !few && direct_ok<T>(a);
@@ -1042,7 +1071,8 @@ int32_t rows_product(GroupedArgs a, hipStream_t strm) {
     }
     const int br = few ? 32 : big ? 256 : kTile, bn = few ? 64 : big ? 256 : kTile;
     a.col_tiles = (a.cols + bn - 1) / bn;
-    const int64_t blocks = (a.rows / br + a.groups + 2) * a.col_tiles;
+    int64_t blocks = (a.rows / br + a.groups + 2) * a.col_tiles;
+    if (!few) blocks = set_run(a, blocks, 2 * a.col_tiles, a.rows / br * a.col_tiles);
     if (blocks > INT32_MAX) return unsupported("grouped linear: more than 2^31 tiles");
     if (few) {
         // workgroups that find rows: at most one per row and column tile. Up to one per CU a workgroup takes
@@ -1079,7 +1109,13 @@ template <typename T, int TILE, int THREADS, bool DIRECT>
 int32_t launch_wgrad(GroupedArgs a, hipStream_t strm) {
     a.row_tiles = (a.out_rows + TILE - 1) / TILE;
     a.col_tiles = (a.cols + TILE - 1) / TILE;
-    const int64_t blocks = a.items * a.row_tiles * a.col_tiles;
+    const int64_t tiles = (int64_t)a.row_tiles * a.col_tiles;
+    const int64_t sure = std::max<int64_t>(a.rows / a.chunk, a.groups) * tiles;
+    // Not for a few tiles, which gain nothing and need an even spread over the XCDs more (a chunk for each place
+    // there is: 36k rows, 6 groups, 602 x 51 fp16 43 us, in runs 52), and not where an XCD gets whole columns of
+    // tiles anyway but could not have all of a chunk's (8k rows, 8 groups, 512 x 2048 bf16 27 us, in runs 31).
+    const bool spread = tiles <= 8 || (a.col_tiles % 8 == 0 && sure / 64 < tiles);
+    const int64_t blocks = set_run(a, a.items * tiles, spread ? 1 : tiles, sure);
     if (blocks > INT32_MAX) return unsupported("grouped linear: more than 2^31 tiles");
     const dim3 grid((unsigned)blocks), block(THREADS);
     if constexpr (TILE == kTile) {

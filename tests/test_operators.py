@@ -789,3 +789,40 @@ def test_graphs_of_the_backward():
     y = mpgnn_amd.grouped_linear(x.detach(), w, ptr)
     dw = torch.autograd.grad(y.sum(), w)[0]
     assert torch.equal(dw, torch.autograd.grad(mpgnn_amd.grouped_linear(x, w, ptr).sum(), w)[0])
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=str)
+@pytest.mark.parametrize("k, n", [(264, 328), (233, 331), (330, 259), (72, 840), (576, 264)])
+def test_grouped_linear_tiles_between(k, n, dt):
+    """Rows and columns enough for tiles of 128 x 128 in each direction, and too few for larger ones: aligned
+    and odd widths, rows of no group, an empty group, a strided x. The 64-bit products run on the GPU."""
+    sizes, before, behind = [1700, 0, 1, 990, 1633, 127], 2, 5
+    g = gen(31)
+    off = offsets(sizes, before)
+    rows, groups = off[-1] + behind, len(sizes)
+    x = rnd(g, rows, k + 8, dtype=dt).to(DEV)[:, 8:]
+    w, b = rnd(g, groups, k, n, scale=k ** -0.5, dtype=dt).to(DEV), rnd(g, groups, n, dtype=dt).to(DEV)
+    dy = rnd(g, rows, n, dtype=dt).to(DEV)
+    leaves = [x.detach().requires_grad_(True), w.clone().requires_grad_(True), b.clone().requires_grad_(True)]
+    y = mpgnn_amd.grouped_linear(leaves[0], leaves[1], torch.tensor(off, device=DEV), leaves[2])
+    got = [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+    for q in range(groups):
+        lo, hi = off[q], off[q + 1]
+        xg, wg, dg, bg = x[lo:hi].double(), w[q].double(), dy[lo:hi].double(), b[q].double()
+        for a, ref, mag, length in [(got[0][lo:hi], xg @ wg + bg, xg.abs() @ wg.abs() + bg.abs(), k),
+                                    (got[1][lo:hi], dg @ wg.t(), dg.abs() @ wg.abs().t(), n),
+                                    (got[2][q], xg.t() @ dg, xg.abs().t() @ dg.abs(), hi - lo)]:
+            assert bool(((a.double() - ref).abs() <= gl_tol(ref, mag, length, dt)).all()), (q, length)
+        ref = dg.sum(0)
+        tol = ((hi - lo) / 16 + 40) * U * dg.abs().sum(0) + half(dt) * ref.abs() + tiny(dt)
+        assert bool(((got[3][q].double() - ref).abs() <= tol).all()), q
+    out = [i for i in range(rows) if i < off[0] or i >= off[-1]]
+    assert float(got[0][out].abs().max()) == 0.0 and float(got[1][out].abs().max()) == 0.0
+    # an infinity and a NaN reach their own row, and the weight's row, alone
+    x[700, 5], x[3000, 9] = math.inf, math.nan
+    y2 = mpgnn_amd.grouped_linear(x, w, torch.tensor(off, device=DEV), b)
+    rest = [i for i in range(rows) if i not in (700, 3000)]
+    assert torch.equal(y2[rest], got[0][rest])
+    assert bool(y2[3000].isnan().all()) and not bool(y2[700].isfinite().any())
+    ref = x[700].double() @ w[0].double() + b[0].double()
+    assert torch.equal(y2[700].double(), ref.to(dt).double())
