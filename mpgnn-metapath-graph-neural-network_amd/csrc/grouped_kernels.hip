@@ -712,7 +712,8 @@ __device__ __forceinline__ void rows_tile(const GroupedArgs& a, const Item& it, 
     }
 }
 
-// A workgroup per row tile and column tile. At 256 rows a group's last tile of at most 128 rows costs half.
+// A workgroup per row tile and column tile. At 256 rows a group's last tile of at most 128 rows costs half, at
+// 128 columns a last one of at most 64 (36k rows, 6 groups, 602 x 51 fp16 41 us, 33 so).
 template <typename T, Layout LB, int BR, int BN, int THREADS, bool DIRECT>
 __global__ __launch_bounds__(THREADS, 2) void grouped_rows_kernel(GroupedArgs a) {
     typedef Product<T, ALONG, LB, BR, BN, THREADS, DIRECT> X;
@@ -726,6 +727,11 @@ __global__ __launch_bounds__(THREADS, 2) void grouped_rows_kernel(GroupedArgs a)
     if constexpr (BR == 256) {
         if (it.hi - r0 <= BR / 2) {
             rows_tile<T, LB, BR / 2, BN, THREADS, DIRECT>(a, it, r0, n0, s0, s1);
+            return;
+        }
+    } else if constexpr (THREADS == 256) {
+        if (a.cols - n0 <= BN / 2) {
+            rows_tile<T, LB, BR, BN / 2, THREADS, DIRECT>(a, it, r0, n0, s0, s1);
             return;
         }
     }
