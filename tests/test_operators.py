@@ -826,3 +826,91 @@ def test_grouped_linear_tiles_between(k, n, dt):
     assert bool(y2[3000].isnan().all()) and not bool(y2[700].isfinite().any())
     ref = x[700].double() @ w[0].double() + b[0].double()
     assert torch.equal(y2[700].double(), ref.to(dt).double())
+
+
+def _one_step(seed, dt):
+    """Norm, grouped product, their gradients and the clipping of these, as one list of tensors."""
+    g = gen(seed)
+    x, w = rnd(g, 300, 72, dtype=dt).to(DEV).requires_grad_(True), rnd(g, 3, 72, 40, dtype=dt).to(DEV).requires_grad_(True)
+    lw, lb = rnd(g, 72, dtype=dt).to(DEV).requires_grad_(True), rnd(g, 72, dtype=dt).to(DEV).requires_grad_(True)
+    ptr = torch.tensor([0, 100, 130, 300], device=DEV)
+    y = mpgnn_amd.grouped_linear(mpgnn_amd.layer_norm(x, lw, lb), w, ptr)
+    grads = torch.autograd.grad(y.float().square().mean(), [x, lw, lb, w])
+    norm, clipped = mpgnn_amd.clip_by_global_norm(grads, 1e-3)
+    return [y.detach(), *grads, norm, *clipped]
+
+
+def test_threads_with_streams_of_their_own():
+    """Several threads call at once (the calls leave the interpreter's lock), each on its own stream."""
+    import threading
+    kinds = [(s, TYPES[s % 3]) for s in range(6)]
+    want = [_one_step(s, dt) for s, dt in kinds]
+    torch.cuda.synchronize()
+    got, errors = [None] * len(kinds), []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(5):
+                    got[i] = _one_step(*kinds[i])
+                torch.cuda.current_stream().synchronize()
+        except Exception as exc:  # noqa: BLE001 - shown by the main thread
+            errors.append(exc)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(kinds))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for a, b in zip(want, got):
+        assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
+def test_checkpointed_and_hooked():
+    """Recomputed activations and saved-tensor hooks (packed to the host) give the same gradients."""
+    from torch.utils.checkpoint import checkpoint
+    g = gen(8)
+    x, w = rnd(g, 50, 24).to(DEV).requires_grad_(True), rnd(g, 2, 24, 17).to(DEV).requires_grad_(True)
+    ptr = torch.tensor([0, 20, 50], device=DEV)
+
+    def f(t):
+        return mpgnn_amd.grouped_linear(mpgnn_amd.layer_norm(t), w, ptr).square().sum()
+
+    want = torch.autograd.grad(f(x), [x, w])
+    again = torch.autograd.grad(checkpoint(f, x, use_reentrant=False), [x, w])
+    with torch.autograd.graph.save_on_cpu():
+        y = f(x)
+    host = torch.autograd.grad(y, [x, w])
+    for other in (again, host):
+        assert all(torch.equal(a, b) for a, b in zip(want, other))
+
+
+def test_odd_arguments():
+    x = torch.ones(4, 8, device=DEV)
+    for bad in (None, [1.0], "x"):
+        with pytest.raises((TypeError, AttributeError)):
+            mpgnn_amd.layer_norm(bad)
+    with pytest.raises(TypeError):
+        mpgnn_amd.layer_norm(x.to_sparse())
+    with pytest.raises(TypeError):
+        mpgnn_amd.clip_by_global_norm([x.to_sparse()], 1.0)
+    with pytest.raises(ValueError):
+        mpgnn_amd.clip_by_global_norm([x], 1.0, out=[])
+    with pytest.raises(ValueError):
+        mpgnn_amd.clip_by_global_norm([x], 1.0, out=[x.half()])
+    with pytest.raises(ValueError):
+        mpgnn_amd.grouped_linear(x, torch.ones(8, 5, device=DEV), torch.tensor([0, 4], device=DEV))
+    assert mpgnn_amd.layer_norm(x, eps=1).dtype == torch.float32
+    # one row, one element, no rows, all leading dimensions
+    assert float(mpgnn_amd.layer_norm(torch.full((1, 1), 7.0, device=DEV))) == 0.0
+    assert mpgnn_amd.layer_norm(torch.zeros(0, 8, device=DEV)).shape == (0, 8)
+    assert mpgnn_amd.layer_norm(torch.zeros(8, device=DEV)).shape == (8,)
+    v = torch.zeros(0, 8, device=DEV, requires_grad=True)
+    lw = torch.ones(8, device=DEV, requires_grad=True)
+    gv, gw = torch.autograd.grad(mpgnn_amd.layer_norm(v, lw).sum(), [v, lw])
+    assert gv.shape == (0, 8) and float(gw.abs().max()) == 0.0
+    w = torch.ones(2, 8, 5, device=DEV, requires_grad=True)
+    y = mpgnn_amd.grouped_linear(v, w, torch.zeros(3, dtype=torch.int64, device=DEV))
+    gv, gw = torch.autograd.grad(y.sum(), [v, w])
+    assert gv.shape == (0, 8) and float(gw.abs().max()) == 0.0
