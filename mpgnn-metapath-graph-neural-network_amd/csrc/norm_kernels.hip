@@ -298,7 +298,6 @@ __global__ __launch_bounds__(RowShape<TPR>::threads) void layer_norm_bwd_kernel(
     // the weight stays in registers, but for the largest teams, whose 128 a thread have no room
     constexpr bool KEEP = TPR < 1024;
     float w[KEEP ? NV : 1][V], dw[NV][V], db[NV][V], dwc[COMP ? NV : 1][V], dbc[COMP ? NV : 1][V];
-    auto weight = [&](int c) { return a.w && c < F ? param_at<T>(a.w, a.w_f32, c) : 1.0f; };
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         if constexpr (KEEP) params_at<T>(w[i], a.w, a.w_f32, (i * TPR + t) * V, F, 1.0f);
@@ -331,17 +330,20 @@ __global__ __launch_bounds__(RowShape<TPR>::threads) void layer_norm_bwd_kernel(
         next_dy.widen(g);
         fetch(r + step);
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+        for (int i = 0; i < NV; ++i) {
+            float wi[V];
+            if constexpr (!KEEP) params_at<T>(wi, a.w, a.w_f32, (i * TPR + t) * V, F, 1.0f);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 if (!(live && R::in(i, j, t, F))) continue;
                 xh[i][j] = (xh[i][j] - mean) * rstd;
                 add_to<COMP>(dw[i][j], dwc[COMP ? i : 0][j], g[i][j] * xh[i][j]);
                 add_to<COMP>(db[i][j], dbc[COMP ? i : 0][j], g[i][j]);
-                g[i][j] *= KEEP ? w[KEEP ? i : 0][j] : weight((i * TPR + t) * V + j);
+                g[i][j] *= KEEP ? w[KEEP ? i : 0][j] : wi[j];
                 s[0] += g[i][j];
                 s[1] = __builtin_fmaf(g[i][j], xh[i][j], s[1]);
             }
+        }
         if (!a.out) continue;
         row_sum<TPR, 2>(s, lds, turn);
         if (!live) continue;
@@ -372,12 +374,16 @@ __global__ __launch_bounds__(RowShape<TPR>::threads) void layer_norm_bwd_kernel(
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < NV; ++i)
+            for (int i = 0; i < NV; ++i) {
+                const int c = (i * TPR + t) * V;
+                if (c + V <= F) {
+                    __builtin_memcpy(pw + (int64_t)k * F + c, d[i], sizeof(d[i]));
+                } else {
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const int c = (i * TPR + t) * V + j;
-                    if (c < F) pw[(int64_t)k * F + c] = d[i][j];
+                    for (int j = 0; j < V; ++j)
+                        if (c + j < F) pw[(int64_t)k * F + c + j] = d[i][j];
                 }
+            }
         }
     }
 }
