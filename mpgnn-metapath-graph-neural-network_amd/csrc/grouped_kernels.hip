@@ -850,7 +850,7 @@ __global__ __launch_bounds__(THREADS, DIRECT ? 2 : 3) void grouped_wgrad_kernel(
     const int bid = tile_of(a);
     const int id = bid / tiles, tile = bid % tiles;
     const Item it = find_item<THREADS>(a, id, a.chunk, 1, false);
-    if (it.group < 0) return;
+    if (it.group < 0 || id >= a.items) return;  // groups that a decreasing ptr makes overlap have more parts than slabs
     const int64_t r0 = (int64_t)(tile / a.col_tiles) * BR, n0 = (int64_t)(tile % a.col_tiles) * BN;
     const int64_t c_lo = it.lo + (int64_t)it.part * a.chunk;
     const int64_t c_hi = c_lo + a.chunk < it.hi ? c_lo + a.chunk : it.hi;

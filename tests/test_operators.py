@@ -914,3 +914,31 @@ def test_odd_arguments():
     y = mpgnn_amd.grouped_linear(v, w, torch.zeros(3, dtype=torch.int64, device=DEV))
     gv, gw = torch.autograd.grad(y.sum(), [v, w])
     assert gv.shape == (0, 8) and float(gw.abs().max()) == 0.0
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=str)
+def test_overlapping_groups_stay_inside_the_workspace(dt):
+    """A ptr that decreases makes groups overlap and have more chunks between them than there are slabs: the
+    weight gradient writes neither behind its workspace nor behind its outputs."""
+    import ctypes
+    from mpgnn_amd import _lib
+    code = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}[dt]
+    g = gen(3)
+    for rows, k, n in ((6000, 40, 24), (6000, 264, 200), (9000, 1200, 600)):
+        x, dy = rnd(g, rows, k, dtype=dt).to(DEV), rnd(g, rows, n, dtype=dt).to(DEV)
+        vals = [0, rows, 100, rows, 7, rows, 0, rows]
+        groups = len(vals) - 1
+        ptr = torch.tensor(vals, device=DEV)
+        need = ctypes.c_int64()
+        assert _lib.lib.mpgnn_grouped_linear_wgrad_workspace_bytes(rows, groups, k, n, ctypes.byref(need)) == 0
+        pad = 1 << 20
+        ws = torch.full((need.value + pad,), 0x5A, dtype=torch.uint8, device=DEV)
+        dw = torch.full((groups * k * n + pad,), 7.0, dtype=dt, device=DEV)
+        db = torch.full((groups * n + pad,), 7.0, dtype=dt, device=DEV)
+        st = _lib.lib.mpgnn_grouped_linear_wgrad(x.data_ptr(), k, dy.data_ptr(), n, rows, code, groups, k, n,
+                                                 ptr.data_ptr(), 64, dw.data_ptr(), db.data_ptr(), ws.data_ptr(),
+                                                 torch.cuda.current_stream().cuda_stream)
+        assert st == 0
+        torch.cuda.synchronize()
+        assert bool((ws[need.value:] == 0x5A).all()) and bool((dw[groups * k * n:] == 7.0).all())
+        assert bool((db[groups * n:] == 7.0).all())
