@@ -13,7 +13,7 @@
 // beside each of these sums, since one thread adds hundreds of rows.
 //
 // Measured, forward and backward with the second kernel (a large copy runs at 4.96 TB/s): 16,384 x 4,096 bf16 51 and
-// 96 + 8 us (5.2 and 4.2 TB/s); 2 M x 256 fp32 811 and 1247 + 9 us (5.0 TB/s); 14,541 x 128 fp32 5.4 and 6.8 + 4.7
+// 96 + 8 us (5.2 and 4.2 TB/s); 2 M x 256 fp32 811 and 1247 + 9 us (5.0 TB/s); 14,541 x 128 fp32 7.6 and 6.8 + 4.4
 // us, launches and latency.
 #include <algorithm>
 
