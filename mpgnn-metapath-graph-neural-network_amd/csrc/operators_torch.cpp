@@ -11,6 +11,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <algorithm>
@@ -43,6 +44,25 @@ int32_t require(const Tensor& t, const char* name) {
     TORCH_CHECK_TYPE(code >= 0, "mpgnn_amd: `", name, "` must be float32, bfloat16 or float16, got ", t.scalar_type());
     TORCH_CHECK_TYPE(t.layout() == at::kStrided, "mpgnn_amd: `", name, "` must be dense, got ", t.layout());
     return code;
+}
+
+// A tangent of forward-mode differentiation would be dropped, and a trace would record the outputs' allocation
+// without the kernel that fills them: both are refused.
+void refuse_tangent(const Tensor& t, const char* what) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(), "mpgnn_amd: ", what,
+                                " has no forward-mode derivative: an argument carries a tangent");
+}
+
+void refuse_tracing(const char* what) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing(), "mpgnn_amd: ", what,
+                                " cannot be recorded by torch.jit.trace");
+}
+
+void refuse_transforms(const char* what, const Tensor& a, const Tensor& b = {}, const Tensor& c = {}) {
+    refuse_tracing(what);
+    refuse_tangent(a, what);
+    refuse_tangent(b, what);
+    refuse_tangent(c, what);
 }
 
 // The C entry points' statuses as the exceptions that _lib.check raises for them.
@@ -138,6 +158,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     }
 
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        refuse_tangent(grads[0], "layer_norm");
         const auto saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &weight = saved[1], &stats = saved[2];
         const int64_t types = ctx->saved_data["types"].toInt(), want = ctx->saved_data["want"].toInt();
@@ -176,6 +197,7 @@ int32_t norm_param(const Tensor& p, const char* name, const Tensor& x, int32_t c
 }
 
 Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias, double eps) {
+    refuse_transforms("layer_norm", x, weight.value_or(Tensor()), bias.value_or(Tensor()));
     const int32_t code = require(x, "x");
     TORCH_CHECK_VALUE(x.dim() > 0 && x.size(-1) > 0,
                       "layer_norm normalises a last dimension of at least one element, got shape ", x.sizes());
@@ -222,6 +244,7 @@ struct GroupedLinear : torch::autograd::Function<GroupedLinear> {
     }
 
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        refuse_tangent(grads[0], "grouped_linear");
         const auto saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &w = saved[1], &ptr = saved[2];
         const Rows r(x), d(grads[0]);
@@ -253,6 +276,7 @@ struct GroupedLinear : torch::autograd::Function<GroupedLinear> {
 };
 
 Tensor grouped_linear(const Tensor& x, const Tensor& weight, const Tensor& ptr, const std::optional<Tensor>& bias) {
+    refuse_transforms("grouped_linear", x, weight, bias.value_or(Tensor()));
     const int32_t code = require(x, "x");
     TORCH_CHECK_VALUE(x.dim() == 2 && weight.dim() == 3 && ptr.dim() == 1,
                       "grouped_linear takes x [rows, K], weight [groups, K, N] and group_ptr [groups + 1], got ",
@@ -294,6 +318,7 @@ std::pair<Tensor, std::vector<Tensor>> clip(const std::vector<Tensor>& grads, st
                                             int64_t scaled, double max_norm, bool largest) {
     const bool in_place = scaled == IN_PLACE, fresh = scaled == OUT && !outs;
     const char* what = in_place ? "gradients" : "tensors";
+    refuse_tracing("clipping");
     const size_t n = grads.size();
     const Tensor& first = grads[0];
     std::vector<mpgnn_clip_tensor> records(n);
@@ -304,6 +329,7 @@ std::pair<Tensor, std::vector<Tensor>> clip(const std::vector<Tensor>& grads, st
     std::vector<const void*> written;
     for (size_t i = 0; i < n; ++i) {
         const Tensor& g = grads[i];
+        refuse_tangent(g, "clipping");
         mpgnn_clip_tensor& r = records[i];
         r.dtype = require(g, what);
         TORCH_CHECK(g.device() == first.device(), what, " are on several devices: ", first.device(), " and ", g.device());

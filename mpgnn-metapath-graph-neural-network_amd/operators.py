@@ -10,7 +10,8 @@ tensors on the GPU (C ABI calls on torch's current stream of the tensors' device
 
 Statistics, sums and matrix accumulators are held in fp32 or wider and a 16-bit result is rounded
 once. Results do not change from run to run. No call synchronises the device or keeps anything
-from one call to the next, so all of them can be captured into a HIP graph.
+from one call to the next, so all of them can be captured into a HIP graph. A forward-mode tangent
+(torch.autograd.forward_ad) on an argument and a recording torch.jit.trace raise NotImplementedError.
 """
 from __future__ import annotations
 

@@ -942,3 +942,25 @@ def test_overlapping_groups_stay_inside_the_workspace(dt):
         torch.cuda.synchronize()
         assert bool((ws[need.value:] == 0x5A).all()) and bool((dw[groups * k * n:] == 7.0).all())
         assert bool((db[groups * n:] == 7.0).all())
+
+
+def test_tangents_and_traces_are_refused_on_the_gpu():
+    """As on the CPU, and for a tangent that the backward meets on the incoming gradient."""
+    from torch.autograd import forward_ad
+    g = gen(91)
+    x, w = rnd(g, 6, 8).to(DEV), rnd(g, 2, 8, 8).to(DEV)
+    ptr = torch.tensor([0, 2, 6], device=DEV)
+    calls = (lambda t: mpgnn_amd.layer_norm(t), lambda t: mpgnn_amd.grouped_linear(t, w, ptr))
+    with forward_ad.dual_level():
+        for f in calls + (lambda t: mpgnn_amd.clip_by_global_norm([w, t], 1.0),):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                f(forward_ad.make_dual(x, x))
+        for f in calls:
+            xg = x.clone().requires_grad_(True)
+            y = f(xg)
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                torch.autograd.grad(y, xg, forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y)))
+    for f in calls + (lambda t: mpgnn_amd.clip_by_global_norm([t], 1.0)[0],):
+        with pytest.raises(NotImplementedError, match="trace"):
+            torch.jit.trace(f, (x,))
+        f(x)  # and nothing is left behind

@@ -115,3 +115,24 @@ def test_modules_match_torch_parameters():
     g = mpgnn_amd.GroupedLinear(6, 4, 3)
     assert tuple(g.weight.shape) == (3, 6, 4) and tuple(g.bias.shape) == (3, 4) and float(g.bias.abs().max()) == 0.0
     assert float(g.weight.abs().max()) <= (6.0 / (6 + 4)) ** 0.5
+
+
+def test_tangents_and_traces_are_refused():
+    """A forward-mode tangent would be lost and a trace would hold no kernel: refused before anything else."""
+    from torch.autograd import forward_ad
+    x, w, ptr = torch.ones(4, 8), torch.ones(2, 8, 5), torch.tensor([0, 2, 4])
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+
+        for f in (lambda: mpgnn_amd.layer_norm(dual(x)), lambda: mpgnn_amd.layer_norm(x, dual(x[0])),
+                  lambda: mpgnn_amd.layer_norm(x, None, dual(x[0])), lambda: mpgnn_amd.layer_norm(dual(x).requires_grad_()),
+                  lambda: mpgnn_amd.grouped_linear(dual(x), w, ptr), lambda: mpgnn_amd.grouped_linear(x, dual(w), ptr),
+                  lambda: mpgnn_amd.grouped_linear(x, w, ptr, dual(w[:, 0])),
+                  lambda: mpgnn_amd.clip_by_global_norm([dual(x)], 1.0)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                f()
+    for f in (lambda t: mpgnn_amd.layer_norm(t), lambda t: mpgnn_amd.grouped_linear(t, w, ptr),
+              lambda t: mpgnn_amd.clip_by_global_norm([t], 1.0)[0]):
+        with pytest.raises(NotImplementedError, match="trace"):
+            torch.jit.trace(f, (x,))
