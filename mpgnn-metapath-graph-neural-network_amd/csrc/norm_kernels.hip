@@ -271,14 +271,14 @@ __global__ __launch_bounds__(RowShape<TPR>::threads) void layer_norm_fwd_kernel(
     }
 }
 
-// a + v with the rounding error carried in c (Kahan's sum); plain for 16-bit inputs, whose outputs
-// round far coarser than the sum
+// a + v with the rounding error carried in c (Kahan's sum; an infinite sum has none, and stays what it
+// is); plain for 16-bit inputs, whose outputs round far coarser than the sum
 template <bool COMP>
 __device__ __forceinline__ void add_to(float& a, float& c, float v) {
     if constexpr (COMP) {
         const float u = v - c;
         const float s = a + u;
-        c = (s - a) - u;
+        c = __builtin_fabsf(s) <= 3.402823466e38f ? (s - a) - u : 0.0f;
         a = s;
     } else {
         a += v;

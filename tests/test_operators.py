@@ -964,3 +964,31 @@ def test_tangents_and_traces_are_refused_on_the_gpu():
         with pytest.raises(NotImplementedError, match="trace"):
             torch.jit.trace(f, (x,))
         f(x)  # and nothing is left behind
+
+
+@pytest.mark.parametrize("rows, f, dt", [(40000, 64, torch.float32), (5000, 771, torch.float32),
+                                         (600, 20001, torch.float32), (600, 20001, torch.bfloat16),
+                                         (5000, 771, torch.bfloat16)], ids=str)
+def test_layer_norm_infinite_gradients_in_the_parameters_sums(rows, f, dt):
+    """Infinities of one sign in a column of dy make its sums infinite, of both signs or a NaN no number, as the
+    formula has it, whatever rows follow them in the same thread; the other columns are as without them."""
+    g = gen(rows + f)
+    x, dy = rnd(g, rows, f, dtype=dt), rnd(g, rows, f, dtype=dt)
+    w, b = torch.ones(f, dtype=dt), torch.zeros(f, dtype=dt)
+    xg, wg, bg = (t.to(DEV).requires_grad_(True) for t in (x, w, b))
+    y = mpgnn_amd.layer_norm(xg, wg, bg)
+    clean = torch.autograd.grad(y, (wg, bg), dy.to(DEV), retain_graph=True)
+    dy[3, 5] = math.inf
+    dy[2, 9] = -math.inf
+    dy[rows - 1, 9] = -math.inf
+    dy[3, 60], dy[11, 60] = math.inf, -math.inf
+    dy[3, 33] = math.nan
+    _, _, dw, db = ln_reference(x, w, b, dy, 1e-5)
+    # dw[9] takes -inf * xhat of two rows and is what their signs make it: infinite or NaN
+    for got, ref, old in zip(torch.autograd.grad(y, (wg, bg), dy.to(DEV)), (dw, db), clean):
+        got = got.double().cpu()
+        cols = [5, 9, 33, 60]
+        assert torch.equal(torch.nan_to_num(got[cols], 1.0, 2.0, 3.0), torch.nan_to_num(ref[cols], 1.0, 2.0, 3.0)), got[cols]
+        rest = torch.ones(f, dtype=torch.bool)
+        rest[cols] = False
+        assert torch.equal(got[rest], old.double().cpu()[rest])
