@@ -992,3 +992,15 @@ def test_layer_norm_infinite_gradients_in_the_parameters_sums(rows, f, dt):
         rest = torch.ones(f, dtype=torch.bool)
         rest[cols] = False
         assert torch.equal(got[rest], old.double().cpu()[rest])
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=str)
+@pytest.mark.parametrize("n", [1, 3, 8, 17, 64, 1000, 9001, 50000])
+def test_clip_norm_is_the_exact_one_rounded(n, dt):
+    """Squares and sums in 64 bits and one rounding to fp32, by at most 2^-24 of the norm (the 64-bit sums of both
+    sides add less than n * 2^-52): small lists, where errors of many vectors do not average out, and large ones."""
+    for seed in range(12):
+        t = rnd(gen(1000 * n + seed), n, scale=10.0 ** (seed % 5 - 2), dtype=dt)
+        ref = float(t.double().square().sum().sqrt())
+        norm, _ = mpgnn_amd.clip_by_global_norm([t.to(DEV)], 1.0)
+        assert abs(float(norm.double()) - ref) <= (U + n * 2.0 ** -51) * ref, (seed, float(norm), ref)
