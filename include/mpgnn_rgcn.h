@@ -326,7 +326,7 @@ int32_t mpgnn_grouped_linear_wgrad(const void* x, int64_t x_pitch, const void* d
 
 /* The global norm over a list of gradient tensors (the 2-norm of all their elements, or the largest
  * |element|) -> *norm, and, if the tensors carry `out`, out = grad * min(1, max_norm / (norm + 1e-6))
- * rounded once (out may be grad: in place; other overlaps are not allowed). What a loop runs
+ * rounded once (out may be grad: in place; an out that overlaps another tensor otherwise is refused). What a loop runs
  * between loss.backward() and optimizer.step() (main.py:1078-1079 has no clipping). Squares are
  * summed in double in a fixed order: bitwise repeatable, no overflow. A NaN or infinite gradient
  * gives the norm and the products that the formula gives. No host synchronisation; the tensor list

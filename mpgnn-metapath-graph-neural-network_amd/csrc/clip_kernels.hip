@@ -18,6 +18,7 @@
 // Measured, norm and scaling: 31 MB of gradients 8.5 + 17.5 us; 400 tensors of 537 MB, four lists, 4 x (39 + 57) us
 // (a read of all of them and a copy at 4.96 TB/s: 324 us).
 #include <algorithm>
+#include <vector>
 
 #include "num_types.h"
 
@@ -258,6 +259,35 @@ int64_t tensor_units(const mpgnn_clip_tensor& t) {
     return (t.numel * dtype_bytes(t.dtype) + kClipUnit - 1) / kClipUnit;
 }
 
+// Does one of the tensors that a launch writes share memory with another that it writes, or with one that it reads
+// other than as a whole in place? Workgroups would then read what others have scaled already.
+bool shared_memory(const mpgnn_clip_tensor* tensors, int32_t n) {
+    struct Range {
+        uintptr_t lo, hi;
+    };
+    std::vector<Range> out;
+    out.reserve(n);
+    auto range = [](const mpgnn_clip_tensor& t, const void* p) {
+        const uintptr_t lo = reinterpret_cast<uintptr_t>(p);
+        return Range{lo, lo + (uintptr_t)(t.numel * dtype_bytes(t.dtype))};
+    };
+    for (int32_t k = 0; k < n; ++k)
+        if (tensors[k].numel > 0) out.push_back(range(tensors[k], tensors[k].out));
+    const auto before = [](const Range& a, const Range& b) { return a.lo < b.lo; };
+    if (!std::is_sorted(out.begin(), out.end(), before)) std::sort(out.begin(), out.end(), before);
+    for (size_t i = 1; i < out.size(); ++i)
+        if (out[i].lo < out[i - 1].hi) return true;
+    for (int32_t k = 0; k < n; ++k) {
+        const mpgnn_clip_tensor& t = tensors[k];
+        if (t.numel == 0 || t.grad == t.out) continue;  // in place: compared with the others above
+        const Range g = range(t, t.grad);
+        // the outputs are apart, so their ends are in order too: the first that ends behind the beginning
+        const auto at = std::upper_bound(out.begin(), out.end(), g.lo, [](uintptr_t v, const Range& r) { return v < r.hi; });
+        if (at != out.end() && at->lo < g.hi) return true;
+    }
+    return false;
+}
+
 template <typename OP>
 int32_t clip_run(const mpgnn_clip_tensor* tensors, int32_t n, float max_norm, int32_t scale, float* norm, void* ws,
                  hipStream_t strm) {
@@ -361,6 +391,16 @@ extern "C" int32_t mpgnn_clip_by_global_norm(const mpgnn_clip_tensor* tensors, i
     if (with_out && with_out != nonempty)
         return arg_error("mpgnn_clip_by_global_norm: out given for some tensors only");
     if (units > INT32_MAX) return unsupported("mpgnn_clip_by_global_norm: over 2^31 units of 16 KB");
+    if (with_out) {
+        try {
+            if (shared_memory(tensors, n))
+                return arg_error("mpgnn_clip_by_global_norm: an out overlaps another tensor of the list (scaled twice, or "
+                                 "read after it was scaled)");
+        } catch (...) {
+            set_last_error_cstr("mpgnn_clip_by_global_norm: out of host memory");
+            return MPGNN_ERR_ALLOC;
+        }
+    }
     hipStream_t strm = static_cast<hipStream_t>(stream);
     const float mn = (float)max_norm;
     return norm_kind == MPGNN_NORM_2 ? clip_run<SumSq>(tensors, n, mn, with_out > 0, norm, workspace, strm)

@@ -326,7 +326,6 @@ std::pair<Tensor, std::vector<Tensor>> clip(const std::vector<Tensor>& grads, st
     if (outs) to = std::move(*outs);
     std::vector<Tensor> copies;                       // of strided gradients
     std::vector<std::pair<size_t, size_t>> back;      // (gradient, its copy) to be written back
-    std::vector<const void*> written;
     for (size_t i = 0; i < n; ++i) {
         const Tensor& g = grads[i];
         refuse_tangent(g, "clipping");
@@ -348,7 +347,6 @@ std::pair<Tensor, std::vector<Tensor>> clip(const std::vector<Tensor>& grads, st
         }
         if (in_place) {
             r.out = const_cast<void*>(r.grad);
-            if (r.numel) written.push_back(g.data_ptr());
         } else if (fresh) {
             to.push_back(at::empty(g.sizes(), g.options()));
             r.out = to.back().data_ptr();
@@ -358,13 +356,17 @@ std::pair<Tensor, std::vector<Tensor>> clip(const std::vector<Tensor>& grads, st
                                   o.device() == g.device() && o.layout() == at::kStrided && o.is_contiguous(),
                               "out must hold contiguous tensors of the inputs' sizes, types and device");
             r.out = o.data_ptr();
-            if (r.numel) written.push_back(r.out);
         }
     }
-    // scaled in place twice, a tensor would be scaled by the factor's square
-    std::sort(written.begin(), written.end());
-    TORCH_CHECK_VALUE(std::adjacent_find(written.begin(), written.end()) == written.end(),
-                      "one tensor is to be scaled twice");
+    // the C entry point refuses tensors that overlap, but of a strided gradient it sees the copy
+    if (!back.empty()) {
+        std::vector<const void*> written;
+        for (const Tensor& g : grads)
+            if (g.numel()) written.push_back(g.data_ptr());
+        std::sort(written.begin(), written.end());
+        TORCH_CHECK_VALUE(std::adjacent_find(written.begin(), written.end()) == written.end(),
+                          "one tensor is to be scaled twice");
+    }
     int64_t size = 0;
     check(mpgnn_clip_workspace_bytes((int32_t)n, &size), "mpgnn_clip_workspace_bytes");
     const Tensor ws = bytes(size, first);

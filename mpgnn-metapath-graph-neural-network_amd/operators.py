@@ -79,7 +79,8 @@ def clip_by_global_norm(tensors, max_norm: float, norm_type: float = 2.0, out=No
     """``(norm, clipped)``: the global norm over ``tensors`` (the 2-norm of all elements, or the largest
     magnitude with ``norm_type=inf``) as an fp32 scalar tensor, and ``t * min(1, max_norm / (norm + 1e-6))``
     of each, in new tensors or in those of ``out`` (same sizes, types and device, contiguous; ``out`` may
-    be ``tensors`` itself, otherwise the two must not overlap). Not differentiable; no host synchronisation.
+    be ``tensors`` itself; one that overlaps another tensor otherwise is refused). Not differentiable; no host
+    synchronisation.
 
     The factor is computed and applied in fp32 and each product rounded once to its tensor's type. An
     infinite or NaN gradient makes the norm so, and the products what the formula gives."""

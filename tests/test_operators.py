@@ -1004,3 +1004,34 @@ def test_clip_norm_is_the_exact_one_rounded(n, dt):
         ref = float(t.double().square().sum().sqrt())
         norm, _ = mpgnn_amd.clip_by_global_norm([t.to(DEV)], 1.0)
         assert abs(float(norm.double()) - ref) <= (U + n * 2.0 ** -51) * ref, (seed, float(norm), ref)
+
+
+def test_clip_overlapping_and_neighbouring_tensors():
+    """Views that share elements with another tensor of the list are refused before anything is written; neighbours in
+    one bucket, and strided slices that interleave, are clipped as tensors of their own."""
+    flat = rnd(gen(92), 4096, scale=3.0).to(DEV)
+    kept = flat.clone()
+    a, b = flat[:1000], flat[1000:3000]
+    for tensors, out in (([flat, a], None), ([b, flat[2999:3001]], None), ([a, b[:1000]], [b[:1000], a]),
+                         ([flat[:64]], [flat[1:65]]), ([a, b], [flat[3000:4000], flat[500:2500]])):
+        with pytest.raises(ValueError, match="overlaps"):
+            if out is None:
+                params = [torch.nn.Parameter(t.clone()) for t in tensors]
+                for p, t in zip(params, tensors):
+                    p.grad = t
+                mpgnn_amd.clip_grad_norm_(params, 1.0)
+            else:
+                mpgnn_amd.clip_by_global_norm(tensors, 1.0, out=out)
+        assert torch.equal(flat, kept)
+    assert mpgnn_amd.clip_by_global_norm([flat, a], 1.0)[1][1].shape == a.shape  # new tensors: the inputs may overlap
+    parts = [flat[:1000], flat[1000:3000], flat[3000:3000], flat[3000:]]
+    norm, _ = mpgnn_amd.clip_by_global_norm(parts[::-1], 1.0, out=parts[::-1])
+    ref = kept.double().cpu()
+    n = float(ref.square().sum().sqrt())
+    # the factor's division and sum, its product with the element and the norm round: five roundings
+    within(flat, ref / (n + 1e-6), 6 * U * ref.abs() / n, "neighbours")
+    grid = kept.view(64, 64).clone()
+    params = [torch.nn.Parameter(torch.zeros(64, 40, device=DEV)), torch.nn.Parameter(torch.zeros(64, 24, device=DEV))]
+    params[0].grad, params[1].grad = grid[:, :40], grid[:, 40:]
+    mpgnn_amd.clip_grad_norm_(params, 1.0)
+    within(grid, (ref / (n + 1e-6)).view(64, 64), (6 * U * ref.abs() / n).view(64, 64), "interleaved")

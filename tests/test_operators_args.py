@@ -136,3 +136,26 @@ def test_tangents_and_traces_are_refused():
               lambda t: mpgnn_amd.clip_by_global_norm([t], 1.0)[0]):
         with pytest.raises(NotImplementedError, match="trace"):
             torch.jit.trace(f, (x,))
+
+
+def test_clip_refuses_overlapping_tensors():
+    """An out that shares memory with another tensor of the list, written or read, would depend on which workgroup
+    comes first: refused on the host (the addresses here are never read)."""
+    def clip(*tensors):
+        arr = (_lib.ClipTensor * len(tensors))()
+        for t, (grad, out, numel, dtype) in zip(arr, tensors):
+            t.grad, t.out, t.numel, t.dtype = grad, out, numel, dtype
+        return lib.mpgnn_clip_by_global_norm(ctypes.addressof(arr), len(tensors), _lib.NORM_2, 1.0, P, P, None)
+
+    a, b, c, f32, bf16 = 1 << 16, 1 << 17, 1 << 18, _lib.F32, _lib.BF16
+    for bad in ([(a, a, 64, f32), (a + 128, a + 128, 8, f32)],            # a bucket and a view into it, in place
+                [(a + 128, a + 128, 8, f32), (a, a, 64, f32)],            # in either order
+                [(a, a, 64, f32), (a, a, 64, f32)],                       # one tensor twice
+                [(a, a, 64, f32), (a, a, 32, f32)],
+                [(a, b, 64, f32), (b, a, 64, f32)],                       # swapped
+                [(a, b, 64, f32), (b + 64, c, 64, f32)],                  # an out over the end of another's input
+                [(a, b, 64, f32), (c, b + 252, 64, f32)],                 # two outs by one element
+                [(a, a + 4, 64, f32)],                                    # its own input, moved by an element
+                [(c, c, 64, bf16), (c + 124, b, 4, bf16)]):               # read while it is scaled
+        assert clip(*bad) == _lib.MPGNN_ERR_ARG, bad
+        assert "overlaps" in lib.mpgnn_last_error().decode()
