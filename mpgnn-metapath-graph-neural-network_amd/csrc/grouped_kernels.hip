@@ -1046,6 +1046,11 @@ bool direct_ok(const GroupedArgs& a) {
            a.b_group % 8 == 0 && a.r_pitch <= reach && a.b_pitch <= reach;
 }
 
+// A launch has at most 2^32 - 1 threads in a dimension.
+constexpr char kTooMany[] = "grouped linear: more tiles (rows / 32 to 256 + groups, times column tiles) than a launch has "
+                            "workgroups";
+bool fits_launch(int64_t blocks, int threads) { return blocks <= (int64_t)UINT32_MAX / threads; }
+
 template <typename T, Layout LB, int WAVES>
 void launch_few(GroupedArgs a, unsigned blocks, hipStream_t strm) {
     hipLaunchKernelGGL((grouped_few_rows_kernel<T, LB, WAVES>), dim3(blocks), dim3(WAVES * 64), 0, strm, a);
@@ -1086,12 +1091,13 @@ int32_t rows_product(GroupedArgs a, hipStream_t strm) {
     a.col_tiles = (a.cols + bn - 1) / bn;
     int64_t blocks = (a.rows / br + a.groups + 2) * a.col_tiles;
     if (!few) blocks = set_run(a, blocks, 2 * a.col_tiles, a.rows / br * a.col_tiles);
-    if (blocks > INT32_MAX) return unsupported("grouped linear: more than 2^31 tiles");
+    // workgroups that find rows: at most one per row and column tile. Up to one per CU a workgroup of the few-rows
+    // kernel takes eight waves, to have as many bytes on their way (of which a CU holds one workgroup, two of four)
+    const int64_t busy = std::min<int64_t>(a.rows, a.rows / br + a.groups) * a.col_tiles;
+    const bool wide = few ? busy <= 256 : big || sizeof(T) == 4;
+    if (!fits_launch(blocks, wide ? 512 : 256)) return unsupported(kTooMany);
     if (few) {
-        // workgroups that find rows: at most one per row and column tile. Up to one per CU a workgroup takes
-        // eight waves, to have as many bytes on their way (of which a CU holds one workgroup, two of four)
-        const int64_t busy = std::min<int64_t>(a.rows, a.rows / br + a.groups) * a.col_tiles;
-        if (busy <= 256) launch_few<T, LB, 8>(a, (unsigned)blocks, strm);
+        if (wide) launch_few<T, LB, 8>(a, (unsigned)blocks, strm);
         else launch_few<T, LB, 4>(a, (unsigned)blocks, strm);
     } else if constexpr (sizeof(T) == 2) {
         if (big) launch_rows<T, LB, 256, 512, true>(a, (unsigned)blocks, strm);
@@ -1129,7 +1135,7 @@ int32_t launch_wgrad(GroupedArgs a, hipStream_t strm) {
     // tiles anyway but could not have all of a chunk's (8k rows, 8 groups, 512 x 2048 bf16 27 us, in runs 31).
     const bool spread = tiles <= 8 || (a.col_tiles % 8 == 0 && sure / 64 < tiles);
     const int64_t blocks = set_run(a, a.items * tiles, spread ? 1 : tiles, sure);
-    if (blocks > INT32_MAX) return unsupported("grouped linear: more than 2^31 tiles");
+    if (!fits_launch(blocks, THREADS)) return unsupported(kTooMany);
     const dim3 grid((unsigned)blocks), block(THREADS);
     if constexpr (TILE == kTile) {
         if (a.dbias) {

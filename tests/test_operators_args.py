@@ -159,3 +159,19 @@ def test_clip_refuses_overlapping_tensors():
                 [(c, c, 64, bf16), (c + 124, b, 4, bf16)]):               # read while it is scaled
         assert clip(*bad) == _lib.MPGNN_ERR_ARG, bad
         assert "overlaps" in lib.mpgnn_last_error().decode()
+
+
+def test_grouped_linear_refuses_more_tiles_than_a_launch_has():
+    """A launch has 2^32 - 1 threads at most: group counts that need more workgroups are refused as unsupported before
+    anything is launched, not by a failed launch (no address here is read)."""
+    for dt in (_lib.F32, _lib.BF16):
+        for rows, groups, n in ((4, 1 << 24, 5), (4, 1 << 24, 1 << 20), (1 << 33, 1, 5), (1 << 30, 1 << 23, 1 << 20)):
+            assert lib.mpgnn_grouped_linear_fwd(P, rows, 8, dt, P, groups, 8, n, None, P, 64, P,
+                                                None) == _lib.MPGNN_ERR_UNSUPPORTED, (rows, groups, n)
+            assert "tiles" in lib.mpgnn_last_error().decode()
+            assert lib.mpgnn_grouped_linear_dgrad(P, rows, 8, dt, P, groups, n, 8, P, 64, P,
+                                                  None) == _lib.MPGNN_ERR_UNSUPPORTED, (rows, groups, n)
+        assert lib.mpgnn_grouped_linear_wgrad(P, 8, P, 5, 4, dt, 1 << 24, 8, 5, P, 64, P, None, P,
+                                              None) == _lib.MPGNN_ERR_UNSUPPORTED
+        assert lib.mpgnn_grouped_linear_wgrad(P, 1 << 22, P, 1 << 22, 4, dt, 1 << 14, 1 << 22, 1 << 22, P, 64, P, None, P,
+                                              None) == _lib.MPGNN_ERR_UNSUPPORTED
