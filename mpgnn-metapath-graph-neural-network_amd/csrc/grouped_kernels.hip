@@ -414,8 +414,9 @@ struct Tile {
                 return (unsigned)((c < left ? c : left - 1) * pitch_ + (idx < end ? idx : end - 8)) * 2;
             }
         }
-        // (Written out, as the compiler would wait for every load before it reads any stage. The wait states are the
-        // ones that m0 needs before a load to LDS and that a scalar from a vector lane needs before a load.)
+        // (Written out, as the compiler would wait for every load before it reads any stage; m0, which holds the place in
+        // LDS, is an operand, so that the compiler knows what is in it. The wait states are the ones that m0 needs before
+        // a load to LDS and that a scalar from a vector lane needs before a load.)
         template <typename F>
         __device__ __forceinline__ void send(E* lds, F&& from) const {
             typedef __attribute__((address_space(3))) E* lptr;
@@ -423,9 +424,9 @@ struct Tile {
             const int64_t origin = scalar((int64_t)base);
 #pragma unroll
             for (int n = 0; n < chunks; ++n)
-                asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1"
+                asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1"
                              :
-                             : "v"(from(n)), "s"(origin), "s"(to + n * THREADS * 16)
+                             : "v"(from(n)), "s"(origin), "{m0}"(to + n * THREADS * 16)
                              : "memory");
         }
         __device__ __forceinline__ void next(E* lds) {

@@ -175,3 +175,14 @@ def test_grouped_linear_refuses_more_tiles_than_a_launch_has():
                                               None) == _lib.MPGNN_ERR_UNSUPPORTED
         assert lib.mpgnn_grouped_linear_wgrad(P, 1 << 22, P, 1 << 22, 4, dt, 1 << 14, 1 << 22, 1 << 22, P, 64, P, None, P,
                                               None) == _lib.MPGNN_ERR_UNSUPPORTED
+
+
+def test_inline_assembly_writes_no_register_behind_the_compiler():
+    """m0 cannot be named as clobbered (the compiler holds it reserved), so no assembly text may write it: it is an
+    operand, "{m0}"."""
+    import os
+    import re
+    src = os.path.join(os.path.dirname(_lib.LIB_PATH), "csrc")
+    texts = [open(os.path.join(src, f)).read() for f in sorted(os.listdir(src)) if f.endswith((".hip", ".h"))]
+    assert any('"{m0}"' in t for t in texts)
+    assert not any(re.search(r"s_\w+ m0\s*,", t) for t in texts)
