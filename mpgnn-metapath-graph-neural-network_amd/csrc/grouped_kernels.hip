@@ -134,18 +134,20 @@ struct Item {
 };
 
 // Item `id` of the list of all groups' parts: each group has ceil(rows / size) of them, at least
-// `least`. With `rest`, the rows before ptr[0] and from ptr[G] on follow as two more groups.
+// `least`. With `rest`, the rows before ptr[0] and from ptr[G] on follow as two more groups. Groups that a
+// decreasing ptr makes overlap have more parts together, but half of the THREADS groups of a turn at most, each no
+// more than a launch has workgroups (2^32 / THREADS): an unsigned count does not wrap around, no two groups get one item.
 template <int THREADS>
 __device__ __forceinline__ Item find_item(const GroupedArgs& a, int id, int size, int least, bool rest) {
-    __shared__ int s_wave[THREADS / 64];
+    __shared__ unsigned s_wave[THREADS / 64];
     __shared__ Item s_item;
     const int n = a.groups + (rest ? 2 : 0);
     if (threadIdx.x == 0) s_item.group = -1;
-    int base = 0;  // parts before g0: the host launches no more than 2^31
+    unsigned base = 0;  // parts before g0
     for (int g0 = 0; g0 < n; g0 += THREADS) {
         const int g = g0 + threadIdx.x;
         int64_t lo = 0, hi = 0;
-        int parts = 0;
+        unsigned parts = 0;
         if (g < a.groups) {
             lo = ptr_at(a, g);
             hi = ptr_at(a, g + 1);
@@ -157,28 +159,28 @@ __device__ __forceinline__ Item find_item(const GroupedArgs& a, int id, int size
             hi = ptr_at(a, 0);
         }
         if (g < n) {
-            parts = (int)((unsigned long long)(hi - lo + size - 1) / (unsigned)size);
-            if (g < a.groups && parts < least) parts = least;
+            parts = (unsigned)((unsigned long long)(hi - lo + size - 1) / (unsigned)size);
+            if (g < a.groups && parts < (unsigned)least) parts = least;
         }
-        int sum = parts;  // inclusive scan over the wave
+        unsigned sum = parts;  // inclusive scan over the wave
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
-            const int v = __shfl_up(sum, d, 64);
+            const unsigned v = __shfl_up(sum, d, 64);
             if ((int)(threadIdx.x % 64) >= d) sum += v;
         }
         if (threadIdx.x % 64 == 63) s_wave[threadIdx.x / 64] = sum;
         __syncthreads();
-        int before = base;
+        unsigned before = base;
 #pragma unroll
         for (int w = 0; w < THREADS / 64; ++w) {
             if (w < (int)(threadIdx.x / 64)) before += s_wave[w];
             base += s_wave[w];
         }
-        const int first = before + sum - parts;
-        if (id >= first && id < first + parts)
-            s_item = Item{g < a.groups ? g : a.groups, id - first, parts, lo, hi};
+        const unsigned end = before + sum, first = end - parts;
+        if ((unsigned)id >= first && (unsigned)id < end)
+            s_item = Item{g < a.groups ? g : a.groups, (int)((unsigned)id - first), (int)parts, lo, hi};
         __syncthreads();
-        if (base > id) break;
+        if (base > (unsigned)id) break;
     }
     Item it = s_item;  // the same in every lane: into scalar registers
     it.group = __builtin_amdgcn_readfirstlane(it.group);
@@ -368,7 +370,6 @@ struct Tile {
             }
             step = L == ALONG ? BK : BK * pitch;
         }
-        __device__ __forceinline__ Walk() {}
         __device__ __forceinline__ void set(int n, const T* p, int64_t pitch, int64_t i, int64_t i_n, int64_t k) {
             if constexpr (L == ALONG) at[n] = p + (i < i_n ? i : i_n - 1) * pitch + k;
             else at[n] = p + k * pitch + (i < i_n ? i : i_n - 8);

@@ -1035,3 +1035,41 @@ def test_clip_overlapping_and_neighbouring_tensors():
     params[0].grad, params[1].grad = grid[:, :40], grid[:, 40:]
     mpgnn_amd.clip_grad_norm_(params, 1.0)
     within(grid, (ref / (n + 1e-6)).view(64, 64), (6 * U * ref.abs() / n).view(64, 64), "interleaved")
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=str)
+@pytest.mark.parametrize("rows, k, n", [(48, 40, 24), (2000, 264, 200), (2001, 233, 331), (30000, 256, 1024)], ids=str)
+def test_decreasing_ptr_stays_inside_the_outputs(rows, k, n, dt):
+    """Groups that overlap because ptr decreases: forward and input gradient write neither before nor behind their
+    outputs (the overlapped rows' values are unspecified)."""
+    from mpgnn_amd import _lib
+    code = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}[dt]
+    g = gen(rows + k)
+    pad = 1 << 16
+    x, dy = rnd(g, rows, k, dtype=dt).to(DEV), rnd(g, rows, n, dtype=dt).to(DEV)
+    for vals in ([0, rows, 0, rows, 0], [rows, 0], [rows // 2, 3, rows, 5, rows + 9, -4], [rows, rows // 3, 1]):
+        groups = len(vals) - 1
+        w = rnd(g, groups, k, n, dtype=dt).to(DEV)
+        for bits, it in ((64, torch.int64), (32, torch.int32)):
+            ptr = torch.tensor(vals, device=DEV, dtype=it)
+            for call, r, width, cols in ((_lib.lib.mpgnn_grouped_linear_fwd, x, k, n),
+                                         (_lib.lib.mpgnn_grouped_linear_dgrad, dy, n, k)):
+                out = torch.full((2 * pad + rows * cols,), 7.0, dtype=dt, device=DEV)
+                bias = (None,) if r is x else ()
+                st = call(r.data_ptr(), rows, width, code, w.data_ptr(), groups, k, n, *bias, ptr.data_ptr(), bits,
+                          out[pad:].data_ptr(), torch.cuda.current_stream().cuda_stream)
+                assert st == _lib.MPGNN_OK
+                torch.cuda.synchronize()
+                assert bool((out[:pad] == 7.0).all()) and bool((out[pad + rows * cols:] == 7.0).all()), (vals, bits)
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=str)
+@pytest.mark.parametrize("off", [0, 1, 2, 3, 5])
+def test_layer_norm_slices_at_every_offset(off, dt):
+    """Column slices that start at any element against the definition, whichever loads their alignment takes."""
+    g = gen(40 + off)
+    rows, f = 65, 264
+    wide = rnd(g, rows, f + 9, scale=2.0, shift=0.5, dtype=dt)
+    ref = ln_reference(wide[:, off:off + f], None, None, None, 1e-5)
+    _, ty = ln_tolerances(wide[:, off:off + f], ref, dt, ln_depth(f))
+    within(mpgnn_amd.layer_norm(wide.to(DEV)[:, off:off + f]), ref[0], ty, off)
