@@ -186,3 +186,25 @@ def test_inline_assembly_writes_no_register_behind_the_compiler():
     texts = [open(os.path.join(src, f)).read() for f in sorted(os.listdir(src)) if f.endswith((".hip", ".h"))]
     assert any('"{m0}"' in t for t in texts)
     assert not any(re.search(r"s_\w+ m0\s*,", t) for t in texts)
+
+
+def test_the_c_library_builds_without_torch():
+    """A host without torch's headers gets the C library and its stamp from the default target, and no module of
+    other sources stays beside it; with them both are built. (What make would run, nothing is built here.)"""
+    import os
+    import shutil
+    import subprocess
+    src = os.path.join(os.path.dirname(_lib.LIB_PATH), "csrc")
+    if shutil.which("make") is None:
+        pytest.skip("no make")
+
+    def commands(*args):
+        out = subprocess.run(["make", "-n", "-B", "-C", src, *args], capture_output=True, text=True, timeout=60)
+        assert out.returncode == 0, out.stderr
+        return out.stdout
+
+    alone = commands("TORCH=")
+    assert "operators_torch" not in alone and "grouped_kernels.hip" in alone and "_srchash.py" in alone
+    assert "rm -f ../_operators.so" in alone
+    both = commands()
+    assert "operators_torch.cpp" in both and "_srchash.py" in both
