@@ -343,6 +343,12 @@ class Net(_FastTrainToggle, torch.nn.Module):
         self.norm1 = LayerNorm(hidden_dim) if layer_norm else None
         self.norm2 = LayerNorm(output_dim) if layer_norm else None
 
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        for name in ("norm1", "norm2"):  # a module pickled before it could have norms
+            if name not in self._modules:
+                self.__dict__.setdefault(name, None)
+
     def forward(self, x, edge_index, edge_type, *, shard=None, group=None, shard_side="gathered"):
         last = self.metapath_length - 1
         stash = None

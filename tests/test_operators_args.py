@@ -208,3 +208,20 @@ def test_the_c_library_builds_without_torch():
     assert "rm -f ../_operators.so" in alone
     both = commands()
     assert "operators_torch.cpp" in both and "_srchash.py" in both
+
+
+def test_net_pickled_before_it_had_norms():
+    """A whole Net saved without the attributes of layer_norm=True loads and runs as one without norms; one with norms
+    keeps them."""
+    import copy
+    import pickle
+    net = mpgnn_amd.Net(4, 8, 2, 8, 3, 2)
+    for name in ("norm1", "norm2"):
+        del net.__dict__[name]
+    old = pickle.loads(pickle.dumps(net))
+    assert old.norm1 is None and old.norm2 is None
+    assert old.state_dict().keys() == mpgnn_amd.Net(4, 8, 2, 8, 3, 2).state_dict().keys()
+    normed = mpgnn_amd.Net(4, 8, 2, 8, 3, 2, layer_norm=True)
+    for again in (pickle.loads(pickle.dumps(normed)), copy.deepcopy(normed)):
+        assert isinstance(again.norm1, mpgnn_amd.LayerNorm) and isinstance(again.norm2, mpgnn_amd.LayerNorm)
+        assert again.state_dict().keys() == normed.state_dict().keys()
