@@ -8,6 +8,7 @@
 #include <ATen/ATen.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -54,8 +55,9 @@ void refuse_tangent(const Tensor& t, const char* what) {
 }
 
 void refuse_tracing(const char* what) {
-    TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing(), "mpgnn_amd: ", what,
-                                " cannot be recorded by torch.jit.trace");
+    TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing() &&
+                                    !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY),
+                                "mpgnn_amd: ", what, " cannot be recorded by torch.jit.trace or make_fx");
 }
 
 void refuse_transforms(const char* what, const Tensor& a, const Tensor& b = {}, const Tensor& c = {}) {

@@ -11,7 +11,7 @@ tensors on the GPU (C ABI calls on torch's current stream of the tensors' device
 Statistics, sums and matrix accumulators are held in fp32 or wider and a 16-bit result is rounded
 once. Results do not change from run to run. No call synchronises the device or keeps anything
 from one call to the next, so all of them can be captured into a HIP graph. A forward-mode tangent
-(torch.autograd.forward_ad) on an argument and a recording torch.jit.trace raise NotImplementedError.
+(torch.autograd.forward_ad) on an argument and a recording torch.jit.trace or make_fx raise NotImplementedError.
 """
 from __future__ import annotations
 

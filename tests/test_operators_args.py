@@ -225,3 +225,15 @@ def test_net_pickled_before_it_had_norms():
     for again in (pickle.loads(pickle.dumps(normed)), copy.deepcopy(normed)):
         assert isinstance(again.norm1, mpgnn_amd.LayerNorm) and isinstance(again.norm2, mpgnn_amd.LayerNorm)
         assert again.state_dict().keys() == normed.state_dict().keys()
+
+
+def test_make_fx_is_refused():
+    """As torch.jit.trace: the graph would hold the outputs' allocation and no kernel."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, w, ptr = torch.ones(4, 8), torch.ones(2, 8, 5), torch.tensor([0, 2, 4])
+    for f in (lambda t: mpgnn_amd.layer_norm(t), lambda t: mpgnn_amd.grouped_linear(t, w, ptr),
+              lambda t: mpgnn_amd.clip_by_global_norm([t], 1.0)[0]):
+        with pytest.raises(NotImplementedError, match="make_fx"):
+            make_fx(f)(x)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):  # and nothing is left behind
+        mpgnn_amd.layer_norm(x)
