@@ -88,18 +88,24 @@ void* data(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 Tensor bytes(int64_t n, const Tensor& like) { return at::empty({n}, like.options().dtype(at::kByte)); }
 
+// A view that negates its memory (the imaginary part of a conjugate) is written out: kernels read memory.
+Tensor as_stored(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+
+Tensor dense(const Tensor& t) { return as_stored(t).contiguous(); }
+
 // A tensor as rows of its last dimension: itself where its rows lie a constant pitch apart (contiguous,
 // or a column slice of a matrix), else a contiguous copy.
 struct Rows {
     Tensor t;
     int64_t rows, pitch;
-    explicit Rows(const Tensor& x) : t(x) {
+    explicit Rows(const Tensor& given) : t(as_stored(given)) {
+        const Tensor& x = t;
         const int64_t width = x.size(-1);
         rows = x.dim() == 2 ? x.size(0) : x.numel() / width;
         pitch = width;
         if (x.is_contiguous()) return;
         if (x.dim() == 2 && x.stride(1) == 1 && x.stride(0) >= width) pitch = x.stride(0);
-        else t = x.contiguous();
+        else t = t.contiguous();
     }
 };
 
@@ -207,14 +213,14 @@ Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight, const st
     Tensor w, b;
     if (weight) {
         wcode = norm_param(*weight, "weight", x, code);
-        w = weight->contiguous();
+        w = dense(*weight);
     }
     if (bias) {
         const int32_t c = norm_param(*bias, "bias", x, code);
         TORCH_CHECK_TYPE(!weight || c == wcode, "weight and bias must have one type, got ", weight->scalar_type(), " and ",
                          bias->scalar_type());
         wcode = c;
-        b = bias->contiguous();
+        b = dense(*bias);
     }
     if (at::GradMode::is_enabled() && (x.requires_grad() || wants_grad(w) || wants_grad(b)))
         return LayerNorm::apply(x, given(w), given(b), eps, (int64_t)code, (int64_t)wcode);
@@ -239,10 +245,10 @@ struct GroupedLinear : torch::autograd::Function<GroupedLinear> {
                           const Tensor& ptr) {
         const Tensor bias = b.value_or(Tensor());
         const Rows r(x);
-        const Tensor w = weight.contiguous();
+        const Tensor w = dense(weight);
         ctx->save_for_backward({r.t, w, ptr});
         ctx->saved_data["want"] = wanted(x, weight, bias);
-        return grouped_forward(r, w, bias.defined() ? bias.contiguous() : bias, ptr);
+        return grouped_forward(r, w, bias.defined() ? dense(bias) : bias, ptr);
     }
 
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -306,7 +312,7 @@ Tensor grouped_linear(const Tensor& x, const Tensor& weight, const Tensor& ptr, 
     const Tensor p = ptr.contiguous();
     if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() || wants_grad(b)))
         return GroupedLinear::apply(x, weight, given(b), p);
-    return grouped_forward(Rows(x), weight.contiguous(), b.defined() ? b.contiguous() : b, p);
+    return grouped_forward(Rows(x), dense(weight), b.defined() ? dense(b) : b, p);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -315,7 +321,7 @@ Tensor grouped_linear(const Tensor& x, const Tensor& weight, const Tensor& ptr, 
 enum Scaled { NONE = 0, OUT = 1, IN_PLACE = 2 };
 
 // The norm of `grads`, and the scaled tensors: none, in `outs` (new ones if there is no list), or in the
-// gradients themselves (strided ones are copied, and copied back).
+// gradients themselves (strided ones and views that negate are copied, and copied back).
 std::pair<Tensor, std::vector<Tensor>> clip(const std::vector<Tensor>& grads, std::optional<std::vector<Tensor>> outs,
                                             int64_t scaled, double max_norm, bool largest) {
     const bool in_place = scaled == IN_PLACE, fresh = scaled == OUT && !outs;
@@ -326,7 +332,7 @@ std::pair<Tensor, std::vector<Tensor>> clip(const std::vector<Tensor>& grads, st
     std::vector<mpgnn_clip_tensor> records(n);
     std::vector<Tensor> to;                           // given or made: where the scaled tensors go
     if (outs) to = std::move(*outs);
-    std::vector<Tensor> copies;                       // of strided gradients
+    std::vector<Tensor> copies;                       // of gradients that are not dense
     std::vector<std::pair<size_t, size_t>> back;      // (gradient, its copy) to be written back
     for (size_t i = 0; i < n; ++i) {
         const Tensor& g = grads[i];
@@ -335,7 +341,7 @@ std::pair<Tensor, std::vector<Tensor>> clip(const std::vector<Tensor>& grads, st
         r.dtype = require(g, what);
         TORCH_CHECK(g.device() == first.device(), what, " are on several devices: ", first.device(), " and ", g.device());
         r.numel = g.numel();
-        if (g.is_contiguous()) {
+        if (g.is_contiguous() && !g.is_neg()) {
             r.grad = g.data_ptr();
         } else {
             if (in_place)
@@ -343,7 +349,7 @@ std::pair<Tensor, std::vector<Tensor>> clip(const std::vector<Tensor>& grads, st
                     TORCH_CHECK_VALUE(g.stride(d) != 0 || g.size(d) < 2,
                                       "a gradient is an expanded tensor, whose elements share memory: it cannot be scaled "
                                       "in place");
-            copies.push_back(g.detach().contiguous());
+            copies.push_back(dense(g.detach()));
             if (in_place) back.emplace_back(i, copies.size() - 1);
             r.grad = copies.back().data_ptr();
         }
@@ -355,7 +361,7 @@ std::pair<Tensor, std::vector<Tensor>> clip(const std::vector<Tensor>& grads, st
         } else if (scaled) {
             const Tensor& o = to[i];
             TORCH_CHECK_VALUE(o.is_cuda() && o.scalar_type() == g.scalar_type() && o.sizes() == g.sizes() &&
-                                  o.device() == g.device() && o.layout() == at::kStrided && o.is_contiguous(),
+                                  o.device() == g.device() && o.layout() == at::kStrided && o.is_contiguous() && !o.is_neg(),
                               "out must hold contiguous tensors of the inputs' sizes, types and device");
             r.out = o.data_ptr();
         }

@@ -1073,3 +1073,32 @@ def test_layer_norm_slices_at_every_offset(off, dt):
     ref = ln_reference(wide[:, off:off + f], None, None, None, 1e-5)
     _, ty = ln_tolerances(wide[:, off:off + f], ref, dt, ln_depth(f))
     within(mpgnn_amd.layer_norm(wide.to(DEV)[:, off:off + f]), ref[0], ty, off)
+
+
+def test_views_that_negate_their_memory():
+    """The imaginary part of a conjugate is a view whose memory holds the negative: as its values, in every place."""
+    g = gen(93)
+    neg = torch._neg_view
+    x, w, b = (rnd(g, *s).to(DEV) for s in ((6, 8), (2, 8, 5), (2, 5)))
+    v, dy, dz = rnd(g, 8).to(DEV), rnd(g, 6, 8).to(DEV), rnd(g, 6, 5).to(DEV)
+    ptr = torch.tensor([0, 2, 6], device=DEV)
+    one = torch.complex(rnd(g, 1), rnd(g, 1)).to(DEV).conj().imag  # contiguous by its only element
+    assert one.is_neg() and one.is_contiguous()
+    norm, (clipped,) = mpgnn_amd.clip_by_global_norm([one], 1e3)
+    assert torch.equal(clipped, one.clone()) and float(norm) == abs(float(one))
+    for t in (x, x[:, 1:7], x.t()):
+        assert torch.equal(mpgnn_amd.layer_norm(neg(t)), mpgnn_amd.layer_norm(-t))
+    assert torch.equal(mpgnn_amd.layer_norm(x, neg(v), neg(v)), mpgnn_amd.layer_norm(x, -v, -v))
+    plain = mpgnn_amd.grouped_linear(-x, -w, ptr, -b)
+    assert torch.equal(mpgnn_amd.grouped_linear(neg(x), neg(w), ptr, neg(b)), plain)
+    for f, d in ((lambda t: mpgnn_amd.layer_norm(t, v), dy), (lambda t: mpgnn_amd.grouped_linear(t, w, ptr), dz)):
+        leaf = x.clone().requires_grad_(True)
+        assert torch.equal(torch.autograd.grad(f(leaf), leaf, neg(d))[0], torch.autograd.grad(f(leaf), leaf, -d)[0])
+        assert torch.equal(torch.autograd.grad(f(neg(leaf)), leaf, d)[0], torch.autograd.grad(f(-leaf), leaf, d)[0])
+    a, c = x.clone(), neg(x.clone())
+    p = [torch.nn.Parameter(x.clone()), torch.nn.Parameter(x.clone())]
+    p[0].grad, p[1].grad = a, c
+    mpgnn_amd.clip_grad_norm_(p, 1.0)
+    assert torch.equal(c, -a) and float(a.abs().max()) < float(x.abs().max())
+    with pytest.raises(ValueError):
+        mpgnn_amd.clip_by_global_norm([x], 1.0, out=[neg(x.clone())])
