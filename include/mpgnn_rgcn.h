@@ -312,7 +312,8 @@ int32_t mpgnn_layer_norm_bwd(const void* dy, int64_t dy_pitch, const void* x, in
  * their rows undefined. Rows in no group (before group_ptr[0], from group_ptr[groups] on) give zero
  * rows of out and dx and take no part in the gradients; an empty group's dweight and dbias are zero.
  * x / dy rows lie x_pitch / dy_pitch elements apart; all else is contiguous, aligned to its elements.
- * fp32 operands run as exact three-way bf16 splits (six products, fp32 accumulation).
+ * fp32 operands run as three-way bf16 splits (six products, fp32 accumulation), exact but for magnitudes below 2^-110,
+ * which lose at most 2^-134 each.
  * MPGNN_ERR_UNSUPPORTED: more than 2^24 columns or groups, or more tiles than a launch has workgroups (2^32 / 256;
  * from about 2^24 groups or 2^31 rows on). */
 int32_t mpgnn_grouped_linear_fwd(const void* x, int64_t rows, int64_t x_pitch, int32_t dtype, const void* weight,

@@ -5,8 +5,8 @@
 // (the second read comes from the 256 MB last-level cache while the list fits it).
 //
 // Each square is taken and summed in double, where no fp32 value's overflows or vanishes: the norm is the exact one
-// rounded once to fp32. (Summing a vector's four or eight squares in fp32 first saves conversions and no time: 31 MB in
-// 7.2 us a kernel either way.) Each thread adds its elements in order, then lanes, waves, workgroups, always in the
+// rounded once to fp32. (Summing a vector's four or eight squares in fp32 first saves conversions and no time: 31 MB
+// in 8.5 us so, 8.0 without.) Each thread adds its elements in order, then lanes, waves, workgroups, always in the
 // same order: the norm does not change from run to run.
 //
 // Two kernels per list of up to kClipMax tensors (the tensor table is the kernel's argument, so a captured
@@ -15,8 +15,8 @@
 // atomic and no third launch. With more than one list, one more workgroup adds the partials of all
 // before the scaling. Tensors of at most kClipSmallBytes together take one launch of one workgroup.
 //
-// Measured, norm and scaling: 31 MB of gradients 8.5 + 17.5 us; 400 tensors of 537 MB, four lists, 4 x (39 + 57) us
-// (a read of all of them and a copy at 4.96 TB/s: 324 us).
+// Measured, norm and scaling, averages: 31 MB of gradients 8.0 + 17.5 us; 400 tensors of 537 MB, four lists, 4 x (41 +
+// 56) us (a read of all of them and a copy at 4.96 TB/s: 324 us).
 #include <algorithm>
 #include <vector>
 

@@ -19,14 +19,17 @@
 //
 // fp32 operands run on the bf16 matrix cores: an exact split of each value in three bf16 pieces
 // and the six products of at least 2^-16 of the full one, which leaves an error of fp32's own
-// size at 16/6 of the fp32 matrix rate. An element whose pieces overflow or are not finite gives a
+// size at 16/6 of the fp32 matrix rate. (Exact from 2^-110 in magnitude on, 8e-34; smaller values lose what lies below
+// the subnormal bf16 numbers, at most 2^-134 each.) An element whose pieces overflow or are not finite gives a
 // result that is not finite; such results are computed again from the operands in fp32, so that
 // infinities and NaN come out as a sum of products has them.
 //
-// Bound by the matrix cores where rows are many (32 groups, 32,768 rows, 2048 x 4096 bf16: forward 627, input
-// gradient 644, weight gradient 725 us, 0.76 to 0.88 of a large library product's rate; 237 groups, 208k rows, 128 x
-// 128 fp32 70, 69 and 67 + 14 us), by reading the weights where they are few (48 rows, 64 groups,
-// 2048 x 2048 bf16 53 us, the hit weights at 4.8 TB/s), by the loads of unaligned rows where widths are odd.
+// Bound by the matrix cores where rows are many (32 groups, 32,768 rows, 2048 x 4096 bf16: forward 598, input gradient
+// 583, weight gradient 660 us on average, 0.82, 0.85 and 0.75 of a large library product's rate; 8 groups, 32,768 rows,
+// 2048 x 2048 fp32: 1369, 1356 and 1383 us, six products at the library's bf16 rate), by splitting and staging the weight
+// for every 128 rows where it is small (237 groups, 208k rows, 128 x 128 fp32 77, 75 and 75 + 15 us), by reading the
+// weights where rows are few (48 rows, 64 groups, 2048 x 2048 bf16 63 us, the hit weights at 4.8 TB/s), by the loads of
+// unaligned rows where widths are odd (20,011 rows, 7 groups, 193 x 301 fp16 20, 22 and 24 + 9 us).
 #include <algorithm>
 
 #include "num_types.h"

@@ -1102,3 +1102,24 @@ def test_views_that_negate_their_memory():
     assert torch.equal(c, -a) and float(a.abs().max()) < float(x.abs().max())
     with pytest.raises(ValueError):
         mpgnn_amd.clip_by_global_norm([x], 1.0, out=[neg(x.clone())])
+
+
+@pytest.mark.parametrize("rows", [9, 700])
+@pytest.mark.parametrize("e, f", [(-100, 60), (-108, 20), (-116, 40), (-126, 60), (60, -126)], ids=str)
+def test_grouped_linear_fp32_small_magnitudes(rows, e, f):
+    """fp32 products of operands near the smallest normal numbers: the third (and second) bf16 piece ends at the
+    subnormal step 2^-133, so that each operand is off by half of that at most on top of the usual error."""
+    g = gen(rows + f)
+    x, dy = rnd(g, rows, 96) * 2.0 ** e, rnd(g, rows, 72) * 2.0 ** e
+    w = rnd(g, 2, 96, 72) * 2.0 ** f
+    off = [0, rows // 3, rows]
+    (y, ym), (dx, dxm), (_, _), _ = gl_reference(x, w, None, off, dy)
+    xg, wg = x.to(DEV).requires_grad_(True), w.to(DEV)
+    got = mpgnn_amd.grouped_linear(xg, wg, torch.tensor(off, device=DEV))
+    got.backward(dy.to(DEV))
+    ones = torch.ones_like
+    (_, ys), (_, dxs), _, _ = gl_reference(ones(x), w, None, off, ones(dy))  # sums of |w|
+    (_, yx), (_, dxd), _, _ = gl_reference(x, ones(w), None, off, dy)        # sums of |x|, of |dy|
+    lost = 2.0 ** -134
+    within(got, y, gl_tol(y, ym, 96, torch.float32) + lost * (ys + yx), "y")
+    within(xg.grad, dx, gl_tol(dx, dxm, 72, torch.float32) + lost * (dxs + dxd), "dx")
