@@ -7,6 +7,7 @@
 // the module at its first call; it links libmpgnn_rgcn.so, the library that _lib.py has checked and loaded.
 #include <ATen/ATen.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/Exceptions.h>
@@ -48,10 +49,12 @@ int32_t require(const Tensor& t, const char* name) {
 }
 
 // A tangent of forward-mode differentiation would be dropped, and a trace would record the outputs' allocation
-// without the kernel that fills them: both are refused.
+// without the kernel that fills them: both are refused. (Not where forward mode is off, as it is inside the forward
+// of a torch.autograd.Function, which answers for the derivative itself.)
 void refuse_tangent(const Tensor& t, const char* what) {
-    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(), "mpgnn_amd: ", what,
-                                " has no forward-mode derivative: an argument carries a tangent");
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !c10::AutogradState::get_tls_state().get_fw_grad_mode() ||
+                                    !t._fw_grad(/*level=*/0).defined(),
+                                "mpgnn_amd: ", what, " has no forward-mode derivative: an argument carries a tangent");
 }
 
 void refuse_tracing(const char* what) {

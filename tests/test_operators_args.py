@@ -237,3 +237,28 @@ def test_make_fx_is_refused():
             make_fx(f)(x)
     with pytest.raises(RuntimeError, match="no CPU fallback"):  # and nothing is left behind
         mpgnn_amd.layer_norm(x)
+
+
+def test_tangents_pass_where_forward_mode_is_off():
+    """Inside the forward of a torch.autograd.Function with a jvp of its own the inputs still carry their tangents:
+    the calls there are not refused for them (here they go on to the next check)."""
+    from torch.autograd import forward_ad
+    w, ptr = torch.ones(2, 8, 5), torch.tensor([0, 2, 4])
+
+    class Own(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, call):
+            return call(x)
+
+        @staticmethod
+        def jvp(ctx, t, _):
+            return t
+
+    with forward_ad.dual_level():
+        x = forward_ad.make_dual(torch.ones(4, 8), torch.ones(4, 8))
+        for call in (lambda t: mpgnn_amd.layer_norm(t), lambda t: mpgnn_amd.grouped_linear(t, w, ptr),
+                     lambda t: mpgnn_amd.clip_by_global_norm([t], 1.0)[0]):
+            with pytest.raises(RuntimeError, match="no CPU fallback"):
+                Own.apply(x, call)
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call(x)
