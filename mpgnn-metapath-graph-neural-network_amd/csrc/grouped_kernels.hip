@@ -4,7 +4,7 @@
 //   weight gradient  dW[g] = x_g^T @ dy_g,  db[g] = the column sums of dy_g
 // with x [M, K] sorted by group, group g owning rows [ptr[g], ptr[g + 1]), W [G, K, N], and ptr on
 // the device: no size is known to the host, so each launch has a workgroup for every tile that
-// there could be (rows / tile + groups), and a workgroup finds its tile by a scan over ptr.
+// there could be (rows / tile + groups), and a workgroup finds its tile by a search over ptr.
 //
 // One kernel computes D[r][n] = sum_c R(r, c) * B(n, c) in tiles on the matrix cores
 // (v_mfma_f32_16x16x32, fp32 accumulators) with either operand stored along c or across it:
@@ -136,55 +136,109 @@ struct Item {
     int64_t lo, hi;
 };
 
+// Groups that start at row `lo`, `before` groups before them, have their places in a list of parts of `size` rows from
+// lo / size + before on: up to the next group's these are one more than the group's rows' whole parts, hence as many as
+// its parts at least, one if it has none, and rows / size + groups in all. No sum of the sizes before is needed.
+__device__ __forceinline__ int64_t place_of(int64_t lo, int size, int64_t before) {
+    return (int64_t)((unsigned long long)lo / (unsigned)size) + before;
+}
+
 // Item `id` of the list of all groups' parts: each group has ceil(rows / size) of them, at least
-// `least`. With `rest`, the rows before ptr[0] and from ptr[G] on follow as two more groups. Groups that a
-// decreasing ptr makes overlap have more parts together, but half of the THREADS groups of a turn at most, each no
-// more than a launch has workgroups (2^32 / THREADS): an unsigned count does not wrap around, no two groups get one item.
+// `least`. With `rest`, the rows before ptr[0] and from ptr[G] on are two more groups.
+//
+// Up to kScanned groups, by a sum over their parts, THREADS groups a turn: the items lie without gaps, and the last
+// workgroups are the idle ones. (Half of the THREADS groups of a turn at most overlap in a decreasing ptr, each no more
+// than a launch has workgroups, 2^32 / THREADS: an unsigned count does not wrap around, no two groups get one item.)
+//
+// Above that by a search over the places, THREADS ways a turn, between which idle workgroups lie. By the sum alone the
+// time grew with the square of the groups: 131,072 groups of a row, 16 x 16 bf16, forward 51.6 ms, 2.3 by the search.
+// us by the sum and by the search, forward:
+//   bf16 (256 threads)   300 groups, 200k rows, 128 x 128  36.6 / 35.0   2,700, 8,192, 64 x 64  48.5 / 28.6
+//   fp32 (512 threads)   520 groups, 200k rows, 128 x 128  64.1 / 70.7   2,700, 300k, 64 x 64   86.1 / 63.0
+//   bf16, tiles of 256   32 groups, 32,768 rows, 2048 x 4096, training   1811 / 1844
+// A ptr that decreases misleads the search; what it finds is still rows inside the tensors, one item a place.
 template <int THREADS>
 __device__ __forceinline__ Item find_item(const GroupedArgs& a, int id, int size, int least, bool rest) {
-    __shared__ unsigned s_wave[THREADS / 64];
+    constexpr int kScanned = THREADS == 512 ? 1024 : THREADS;
+    __shared__ unsigned s_count[2][THREADS / 64];
     __shared__ Item s_item;
     const int n = a.groups + (rest ? 2 : 0);
+    auto parts_of = [&](int64_t lo, int64_t hi) {
+        const unsigned parts = (unsigned)((unsigned long long)(hi - lo + size - 1) / (unsigned)size);
+        return parts < (unsigned)least ? (unsigned)least : parts;
+    };
     if (threadIdx.x == 0) s_item.group = -1;
-    unsigned base = 0;  // parts before g0
-    for (int g0 = 0; g0 < n; g0 += THREADS) {
-        const int g = g0 + threadIdx.x;
-        int64_t lo = 0, hi = 0;
-        unsigned parts = 0;
-        if (g < a.groups) {
-            lo = ptr_at(a, g);
-            hi = ptr_at(a, g + 1);
-            hi = hi < lo ? lo : hi;
-        } else if (g == a.groups) {
-            lo = ptr_at(a, a.groups);
-            hi = a.rows;
-        } else {
-            hi = ptr_at(a, 0);
-        }
-        if (g < n) {
-            parts = (unsigned)((unsigned long long)(hi - lo + size - 1) / (unsigned)size);
-            if (g < a.groups && parts < (unsigned)least) parts = least;
-        }
-        unsigned sum = parts;  // inclusive scan over the wave
+    if (n <= kScanned) {
+        unsigned base = 0;  // parts before g0
+        for (int g0 = 0; g0 < n; g0 += THREADS) {
+            const int g = g0 + threadIdx.x;
+            int64_t lo = 0, hi = 0;
+            if (g < a.groups) {
+                lo = ptr_at(a, g);
+                hi = ptr_at(a, g + 1);
+                hi = hi < lo ? lo : hi;
+            } else if (g == a.groups) {
+                lo = ptr_at(a, a.groups);
+                hi = a.rows;
+            } else {
+                hi = ptr_at(a, 0);
+            }
+            const unsigned parts = g < n ? parts_of(lo, hi) : 0;
+            unsigned sum = parts;  // inclusive scan over the wave
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const unsigned v = __shfl_up(sum, d, 64);
-            if ((int)(threadIdx.x % 64) >= d) sum += v;
-        }
-        if (threadIdx.x % 64 == 63) s_wave[threadIdx.x / 64] = sum;
-        __syncthreads();
-        unsigned before = base;
+            for (int d = 1; d < 64; d <<= 1) {
+                const unsigned v = __shfl_up(sum, d, 64);
+                if ((int)(threadIdx.x % 64) >= d) sum += v;
+            }
+            unsigned* s_sum = s_count[g0 / THREADS % 2];
+            if (threadIdx.x % 64 == 63) s_sum[threadIdx.x / 64] = sum;
+            __syncthreads();  // (of two buffers in turn: one barrier a turn is enough)
+            unsigned before = base;
 #pragma unroll
-        for (int w = 0; w < THREADS / 64; ++w) {
-            if (w < (int)(threadIdx.x / 64)) before += s_wave[w];
-            base += s_wave[w];
+            for (int w = 0; w < THREADS / 64; ++w) {
+                if (w < (int)(threadIdx.x / 64)) before += s_sum[w];
+                base += s_sum[w];
+            }
+            const unsigned end = before + sum, first = end - parts;
+            if ((unsigned)id >= first && (unsigned)id < end)
+                s_item = Item{g < a.groups ? g : a.groups, (int)((unsigned)id - first), (int)parts, lo, hi};
+            if (base > (unsigned)id) break;
         }
-        const unsigned end = before + sum, first = end - parts;
-        if ((unsigned)id >= first && (unsigned)id < end)
-            s_item = Item{g < a.groups ? g : a.groups, (int)((unsigned)id - first), (int)parts, lo, hi};
-        __syncthreads();
-        if (base > (unsigned)id) break;
+    } else {
+        auto start = [&](int h) -> int64_t {  // the first row of entry h, and of the one behind the last
+            if (!rest) return ptr_at(a, h);
+            return h == 0 ? 0 : h <= a.groups + 1 ? ptr_at(a, h - 1) : a.rows;
+        };
+        int lo = 0, hi = n;  // the entry is in [lo, hi)
+        for (int turn = 0;; turn ^= 1) {
+            const int step = (int)(((unsigned)(hi - lo) + THREADS - 1) / THREADS);
+            const int h = lo + (int)threadIdx.x * step;  // below 2^24 + 512 * 2^16
+            const int64_t row = h < hi ? start(h) : 0;
+            const bool begun = h < hi && place_of(row, size, h) <= id;
+            const unsigned long long lanes = __ballot(begun);
+            if (threadIdx.x % 64 == 0) s_count[turn][threadIdx.x / 64] = __popcll(lanes);
+            __syncthreads();  // (of two buffers in turn: one barrier a turn is enough)
+            int count = 0;
+#pragma unroll
+            for (int w = 0; w < THREADS / 64; ++w) count += (int)s_count[turn][w];
+            count = __builtin_amdgcn_readfirstlane(count);
+            if (count == 0) break;
+            lo += (count - 1) * step;
+            if (step == 1) {
+                if ((int)threadIdx.x == count - 1) {
+                    int64_t end = start(h + 1);
+                    end = end < row ? row : end;
+                    const int64_t part = id - place_of(row, size, h);
+                    const unsigned parts = parts_of(row, end);
+                    if (part >= 0 && part < parts)
+                        s_item = Item{!rest ? h : h == 0 || h > a.groups ? a.groups : h - 1, (int)part, (int)parts, row, end};
+                }
+                break;
+            }
+            hi = hi - lo < step ? hi : lo + step;
+        }
     }
+    __syncthreads();
     Item it = s_item;  // the same in every lane: into scalar registers
     it.group = __builtin_amdgcn_readfirstlane(it.group);
     it.part = __builtin_amdgcn_readfirstlane(it.part);
@@ -855,7 +909,7 @@ __global__ __launch_bounds__(THREADS, DIRECT ? 2 : 3) void grouped_wgrad_kernel(
     const int bid = tile_of(a);
     const int id = bid / tiles, tile = bid % tiles;
     const Item it = find_item<THREADS>(a, id, a.chunk, 1, false);
-    if (it.group < 0 || id >= a.items) return;  // groups that a decreasing ptr makes overlap have more parts than slabs
+    if (it.group < 0) return;
     const int64_t r0 = (int64_t)(tile / a.col_tiles) * BR, n0 = (int64_t)(tile % a.col_tiles) * BN;
     const int64_t c_lo = it.lo + (int64_t)it.part * a.chunk;
     const int64_t c_hi = c_lo + a.chunk < it.hi ? c_lo + a.chunk : it.hi;
@@ -885,7 +939,8 @@ __global__ __launch_bounds__(THREADS, DIRECT ? 2 : 3) void grouped_wgrad_kernel(
     });
     const int64_t size = (int64_t)a.out_rows * a.cols;
     const int64_t slab = size + (BIAS ? a.cols : 0);
-    float* part = it.parts > 1 ? a.slabs + (int64_t)id * slab : nullptr;
+    // the slab at the part's place: there are a.items of them, and no group, wherever ptr leads, has a place behind them
+    float* part = it.parts > 1 ? a.slabs + (place_of(it.lo, a.chunk, it.group) + it.part) * slab : nullptr;
     auto again = [&](int64_t row, int64_t col) {
         float v = 0.0f;
         for (int64_t c = c_lo; c < c_hi; ++c)
@@ -945,28 +1000,14 @@ __global__ __launch_bounds__(THREADS, DIRECT ? 2 : 3) void grouped_wgrad_kernel(
 // dW[g] (and db[g]) of the groups cut in chunks: their slabs added in order
 template <typename T>
 __global__ __launch_bounds__(kGlThreads) void grouped_slabs_kernel(GroupedArgs a, int pieces) {
-    __shared__ int64_t s_first;
     const int g = blockIdx.x / pieces;
     const int64_t lo = ptr_at(a, g), hi = ptr_at(a, g + 1);
     if (hi - lo <= a.chunk) return;
-    int64_t parts = (hi - lo + a.chunk - 1) / a.chunk;
-    // items before this group
-    if (threadIdx.x == 0) s_first = 0;
-    __syncthreads();
-    int64_t before = 0;
-    for (int q = threadIdx.x; q < g; q += kGlThreads) {
-        const int64_t l = ptr_at(a, q), h = ptr_at(a, q + 1);
-        const int64_t n = (h - l + a.chunk - 1) / a.chunk;
-        before += n < 1 ? 1 : n;
-    }
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) before += __shfl_xor(before, d, 64);
-    if (threadIdx.x % 64 == 0) atomicAdd((unsigned long long*)&s_first, (unsigned long long)before);  // whole numbers
-    __syncthreads();
+    const int64_t first = place_of(lo, a.chunk, g);
+    // (all of them are inside the workspace, wherever ptr leads: first + parts <= hi / chunk + 1 + g <= items)
+    const int64_t parts = (hi - lo + a.chunk - 1) / a.chunk;
     const int64_t size = (int64_t)a.out_rows * a.cols, slab = size + (a.dbias ? a.cols : 0);
-    const float* p = a.slabs + s_first * slab;
-    parts = min(parts, a.items - s_first);  // short only where ptr decreases and groups overlap
-    if (parts < 1) return;
+    const float* p = a.slabs + first * slab;
     for (int64_t e = ((int64_t)(blockIdx.x % pieces) * kGlThreads + threadIdx.x) * 4; e < slab;
          e += (int64_t)pieces * kGlThreads * 4) {
         const int valid = slab - e < 4 ? (int)(slab - e) : 4;

@@ -1123,3 +1123,44 @@ def test_grouped_linear_fp32_small_magnitudes(rows, e, f):
     lost = 2.0 ** -134
     within(got, y, gl_tol(y, ym, 96, torch.float32) + lost * (ys + yx), "y")
     within(xg.grad, dx, gl_tol(dx, dxm, 72, torch.float32) + lost * (dxs + dxd), "dx")
+
+
+@pytest.mark.parametrize("dt", TYPES, ids=str)
+@pytest.mark.parametrize("groups, rows, bits", [(253, 1000, 64), (254, 9000, 32), (255, 5, 64), (256, 9000, 64),
+                                                (257, 3000, 32), (510, 40000, 64), (513, 700, 64), (2700, 8192, 64),
+                                                (70001, 50000, 32), (1 << 20, 300000, 64)], ids=str)
+def test_grouped_linear_many_groups(groups, rows, bits, dt):
+    """Group counts around the ways of the search for a workgroup's tile and far above them: uneven groups, many empty,
+    rows before the first and behind the last. A million of them ends as soon as any other call."""
+    k, n = 8, 5
+    g = gen(groups + rows)
+    sizes = torch.bincount(torch.randint(0, groups, (rows - 3,), generator=g) ** 2 // groups, minlength=groups)
+    before = 2
+    ptr = torch.cat([torch.tensor([before]), before + sizes.cumsum(0)])
+    x, w, b, dy = (rnd(g, *s, dtype=dt) for s in ((rows, k), (groups, k, n), (groups, n), (rows, n)))
+    of = torch.repeat_interleave(torch.arange(groups), sizes)  # the group of each of the rows that have one
+    lo, hi = before, before + len(of)
+    xd, wd, dd = x.double()[lo:hi], w.double()[of], dy.double()[lo:hi]
+
+    def rows_of(t):  # zeros for the rows of no group
+        out = torch.zeros(rows, t.shape[1], dtype=torch.float64)
+        out[lo:hi] = t
+        return out
+
+    def sums_of(t):
+        return torch.zeros(groups, *t.shape[1:], dtype=torch.float64).index_add_(0, of, t)
+
+    prod = xd[:, :, None] * wd
+    bd = b.double()[of]
+    xg, wg, bg = (t.to(DEV).requires_grad_(True) for t in (x, w, b))
+    y = mpgnn_amd.grouped_linear(xg, wg, ptr.to(DEV, torch.int64 if bits == 64 else torch.int32), bg)
+    y.backward(dy.to(DEV))
+    within(y, rows_of(prod.sum(1) + bd), gl_tol(rows_of(prod.sum(1) + bd), rows_of(prod.abs().sum(1) + bd.abs()), k, dt), "y")
+    back = dd[:, None, :] * wd
+    within(xg.grad, rows_of(back.sum(2)), gl_tol(rows_of(back.sum(2)), rows_of(back.abs().sum(2)), n, dt), "dx")
+    outer = xd[:, :, None] * dd[:, None, :]
+    longest = int(sizes.max())
+    dw, dwm = sums_of(outer), sums_of(outer.abs())
+    within(wg.grad, dw, gl_tol(dw, dwm, longest, dt), "dw")
+    db, dbm = sums_of(dd), sums_of(dd.abs())
+    within(bg.grad, db, longest * U * dbm + half(dt) * db.abs() + tiny(dt), "db")
