@@ -363,6 +363,7 @@ std::pair<Tensor, std::vector<Tensor>> clip(const std::vector<Tensor>& grads, st
             r.out = to.back().data_ptr();
         } else if (scaled) {
             const Tensor& o = to[i];
+            refuse_tangent(o, "clipping");
             TORCH_CHECK_VALUE(o.is_cuda() && o.scalar_type() == g.scalar_type() && o.sizes() == g.sizes() &&
                                   o.device() == g.device() && o.layout() == at::kStrided && o.is_contiguous() && !o.is_neg(),
                               "out must hold contiguous tensors of the inputs' sizes, types and device");

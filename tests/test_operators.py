@@ -1164,3 +1164,14 @@ def test_grouped_linear_many_groups(groups, rows, bits, dt):
     within(wg.grad, dw, gl_tol(dw, dwm, longest, dt), "dw")
     db, dbm = sums_of(dd), sums_of(dd.abs())
     within(bg.grad, db, longest * U * dbm + half(dt) * db.abs() + tiny(dt), "db")
+
+
+def test_clip_refuses_an_out_with_a_tangent():
+    """What is written would keep the tangent of what it held before."""
+    from torch.autograd import forward_ad
+    x = rnd(gen(94), 6, 8).to(DEV)
+    with forward_ad.dual_level():
+        o = forward_ad.make_dual(torch.zeros_like(x), torch.ones_like(x))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            mpgnn_amd.clip_by_global_norm([x], 1.0, out=[o])
+        assert float(forward_ad.unpack_dual(o).primal.abs().max()) == 0.0
